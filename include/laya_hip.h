@@ -228,6 +228,28 @@ int laya_type_embedding_bwd(laya_ctx* ctx, const float* dstates, const int* qtyp
 int laya_softmax_ce_bwd(laya_ctx* ctx, const float* logits, const float* targets, const int* option_offsets,
                         int n_items, float ce_weight, float scale, float* grad, float* loss);
 
+/* Softmax cross entropy of hidden states over a vocabulary (masked-token training and scoring against the tied
+ * embedding table; no counterpart in the reference, whose objective has a few options an item). The logits are never
+ * held: z = x·Wᵀ + b is computed a piece of the vocabulary at a time. For x [rows, hidden], W [vocab, hidden], b [vocab]
+ * (may be NULL) and targets [rows]:
+ *   row_loss[r] = lse[r] − z[r, targets[r]], lse[r] = log Σ_v exp z[r, v], loss = scale·Σ_r row_weights[r]·row_loss[r].
+ * A target of LAYA_NO_LABEL carries no label: its row is not read, row_loss and lse are 0, its gradient is 0 and the
+ * products run on the other rows only. A target outside [0, vocab) otherwise counts in *bad_count (device int32, may
+ * be NULL; written) and is treated alike. row_weights [rows] (≥ 0) may be NULL (1), loss (device float) may be NULL.
+ * W16: W's values as bf16 bit patterns [vocab, hidden], read instead of W (which may then be NULL).
+ * b[v] = −∞ leaves entry v out. Products are fp32-accurate two-piece fp16 products under every matmul precision
+ * (two matrix-core products each with W16, whose values are one piece, three otherwise), scaled by W's and x's rows. */
+#define LAYA_NO_LABEL (-100)
+int laya_vocab_ce_fwd(laya_ctx* ctx, const float* x, int rows, int hidden, const float* W, const uint16_t* W16,
+                      int vocab, const float* b, const int* targets, const float* row_weights, float scale,
+                      float* row_loss, float* lse, float* loss, int* bad_count);
+/* Its gradient from the forward's lse: with G[r, v] = scale·row_weights[r]·(exp(z[r, v] − lse[r]) − [v = targets[r]]),
+ * dx = G·W (OVERWRITE), dW += Gᵀ·x, db += Σ_r G (each skipped when NULL). The sums over rows and over the vocabulary
+ * run in a fixed order. */
+int laya_vocab_ce_bwd(laya_ctx* ctx, const float* x, int rows, int hidden, const float* W, const uint16_t* W16,
+                      int vocab, const float* b, const int* targets, const float* row_weights, float scale,
+                      const float* lse, float* dx, float* dW, float* db);
+
 /* RlcdObjective.Compute (RlcdObjective.cs:57-155) with supplied draws, all operands on the device:
  * option_offsets [n_items + 1] and qtypes [n_items] (int), logits / targets [total_options], draws
  * [groups][total_options] (double); grad [total_options] = ∂loss/∂logit · scale; losses [4] (double):

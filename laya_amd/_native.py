@@ -122,6 +122,8 @@ SIGNATURES = {
     "laya_type_embedding_bwd": (c_int, [P, P, P, c_int, c_int, P]),
     "laya_scatter_add_rows": (c_int, [P, P, P, c_int, c_int, P]),
     "laya_softmax_ce_bwd": (c_int, [P, P, P, P, c_int, c_float, c_float, P, P]),
+    "laya_vocab_ce_fwd": (c_int, [P, P, c_int, c_int, P, P, c_int, P, P, P, c_float, P, P, P, P]),
+    "laya_vocab_ce_bwd": (c_int, [P, P, c_int, c_int, P, P, c_int, P, P, P, c_float, P, P, P, P]),
     "laya_rlcd_objective": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, P, c_double, c_double, c_double,
                                     c_double, c_double, P, P]),
     "laya_grad_norm": (c_int, [P, P, c_size, c_double, P, P]),

@@ -137,6 +137,21 @@ void free_rotary(laya_ctx* ctx, laya_rotary* r) {
 
 static void require_ctx(laya_ctx* ctx) { LAYA_REQUIRE(ctx != nullptr, "null context"); }
 
+// The context's device as the current one for a call, the caller's own restored behind it.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(laya_ctx* ctx) {
+        LAYA_HIP(hipGetDevice(&before));
+        if (before == ctx->device)
+            before = -1;
+        else
+            LAYA_HIP(hipSetDevice(ctx->device));
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
 extern "C" {
 
 const char* laya_last_error(void) { return g_last_error.c_str(); }
@@ -861,6 +876,42 @@ int laya_softmax_ce_bwd(laya_ctx* ctx, const float* logits, const float* targets
     return guarded([&] {
         require_ctx(ctx);
         softmax_ce_bwd(ctx, logits, targets, option_offsets, n_items, ce_weight, scale_, grad, loss);
+    });
+}
+
+static VocabArgs vocab_args(laya_ctx* ctx, const float* x, int rows, int hidden, const float* W, const uint16_t* W16,
+                            int vocab, const float* b, const int* targets, const float* row_weights, float scale) {
+    require_ctx(ctx);
+    LAYA_REQUIRE(rows >= 0 && hidden > 0 && vocab > 0, "vocab_ce: bad size");
+    LAYA_REQUIRE(rows <= 1 << 22 && hidden <= 1 << 16 && vocab <= 1 << 24,
+                 "vocab_ce: at most 2^22 rows, a width of 2^16 and 2^24 vocabulary entries");
+    LAYA_REQUIRE(W || W16, "vocab_ce: null weight");
+    LAYA_REQUIRE(rows == 0 || (x && targets), "vocab_ce: null tensor");
+    LAYA_REQUIRE(std::isfinite(scale), "vocab_ce: scale must be finite");
+    return {x, rows, hidden, W16 ? nullptr : W, reinterpret_cast<const __bf16*>(W16), vocab, b, targets, row_weights,
+            scale};
+}
+
+int laya_vocab_ce_fwd(laya_ctx* ctx, const float* x, int rows, int hidden, const float* W, const uint16_t* W16,
+                      int vocab, const float* b, const int* targets, const float* row_weights, float scale_,
+                      float* row_loss, float* lse, float* loss, int* bad_count) {
+    return guarded([&] {
+        const VocabArgs a = vocab_args(ctx, x, rows, hidden, W, W16, vocab, b, targets, row_weights, scale_);
+        LAYA_REQUIRE(rows == 0 || (row_loss && lse), "vocab_ce: null output");
+        DeviceScope device(ctx);
+        vocab_ce_fwd(ctx, a, row_loss, lse, loss, bad_count);
+    });
+}
+
+int laya_vocab_ce_bwd(laya_ctx* ctx, const float* x, int rows, int hidden, const float* W, const uint16_t* W16,
+                      int vocab, const float* b, const int* targets, const float* row_weights, float scale_,
+                      const float* lse, float* dx, float* dW, float* db) {
+    return guarded([&] {
+        const VocabArgs a = vocab_args(ctx, x, rows, hidden, W, W16, vocab, b, targets, row_weights, scale_);
+        LAYA_REQUIRE(rows == 0 || lse, "vocab_ce: null lse");
+        LAYA_REQUIRE(dx == nullptr || dx != x, "vocab_ce: dx may not be x");
+        DeviceScope device(ctx);
+        vocab_ce_bwd(ctx, a, lse, dx, dW, db);
     });
 }
 

@@ -74,6 +74,16 @@ struct LaunchRecord {
     double flops, bytes;
 };
 
+// Arrays laid one after another, each from a multiple of 256 bytes: `bytes` so far, addresses once `base` is known.
+struct Carve {
+    char* base = nullptr;
+    size_t bytes = 0;
+    template <typename T> void take(T*& p, size_t n) {
+        p = reinterpret_cast<T*>(base + bytes);
+        bytes += (n * sizeof(T) + 255) / 256 * 256;
+    }
+};
+
 }  // namespace laya
 
 // One context: a device, one stream, an allocation ledger and reusable scratch.
@@ -82,7 +92,7 @@ struct laya_ctx {
     hipStream_t stream = nullptr;
     size_t cap = 0, in_use = 0;
     std::unordered_map<void*, size_t> allocations;
-    laya::Workspace scratch[9];
+    laya::Workspace scratch[11];
     hipEvent_t timers[16][2] = {};
     int cu_count = 256;
     bool profiling = false;
@@ -356,6 +366,32 @@ const unsigned* operand_amax_ref(laya_ctx* ctx, AmaxRef r, const float* x, int r
 // The same for two arrays of whole rows (ld = cols), what there is to measure in one launch.
 void operand_amax_refs(laya_ctx* ctx, AmaxRef ra, const float* a, int rows_a, int cols_a, const unsigned** word_a,
                        AmaxRef rb, const float* b, int rows_b, int cols_b, const unsigned** word_b);
+
+// The arrays that `layout` takes, in the context's workspace `slot`.
+constexpr int VOCAB_SLOT = 9, MUON_SLOT = 10;
+template <class F> void carve(laya_ctx* ctx, int slot, F&& layout) {
+    Carve c;
+    layout(c);
+    Carve at;
+    at.base = static_cast<char*>(ctx->workspace(slot, c.bytes));
+    layout(at);
+}
+
+// Cross entropy over a vocabulary (vocab.hip): x [rows, hidden], W [vocab, hidden] or its bf16 values W16, bias and
+// row_weights or null.
+struct VocabArgs {
+    const float* x;
+    int rows, hidden;
+    const float* W;
+    const __bf16* W16;
+    int vocab;
+    const float* bias;
+    const int* targets;
+    const float* row_weights;
+    float scale;
+};
+void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count);
+void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db);
 
 // Σ over rows of a [rows, n] matrix added into out[n], deterministic (bias gradients); amax (optional): max|x| folded
 // into that word group in the same pass. Returns whether it was: only the float4 path of more than 256 rows does.

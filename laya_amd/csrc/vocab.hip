@@ -1,0 +1,833 @@
+// Softmax cross entropy of hidden states over a vocabulary, with its gradient, in pieces of the vocabulary.
+//
+//   z_tv = W_v·x_t + b_v,   L_t = log Σ_v exp z_tv − z_t,y_t,   loss = Σ_t w_t·L_t
+//   G_tv = exp(z_tv − lse_t) − [v = y_t],   dx_t = w_t·Σ_v G_tv·W_v,   dW_v += Σ_t G_tv·(w_t·x_t),   db_v += Σ_t w_t·G_tv
+//
+// The logits are never kept: the forward reduces each tile of them to a maximum and a sum of exponentials a row, merged
+// at the end; the backward computes a piece's logits again and keeps its G as packed fp16 pieces (packed.hpp) just long
+// enough for the piece's two products. Rows without a label are dropped first (label_rows), so that a batch with labels
+// on 15 % of its tokens costs the products of those alone.
+//
+// Scales of the two-piece products (powers of two, so that scaling is exact): W by row (2^ea[v]), x by row (2^ex[t]);
+// G by 2^14. Where the product runs over v, G carries 2^(emin − ea[v]) beside it, which brings W's rows back to one
+// scale; where it runs over t, w_t·x_t has one scale for all.
+#include "elementwise.hpp"
+#include "packed.hpp"
+
+namespace laya {
+namespace {
+
+using namespace packed;
+
+constexpr int TILE = 256;            // logits, G and both gradient products run on 256 x 256 tiles
+constexpr int G_SCALE = 14;          // |G| ≤ 1
+constexpr int MAX_SPLITS = 16;       // ways of dx's sum over a piece of the vocabulary
+constexpr size_t PIECE_BYTES = (size_t)2 << 30;  // of packed table and G that a piece of the vocabulary may take
+constexpr float LOG2E = 1.44269504088896341f;
+
+// Words of a call: [0] labelled rows, [1] targets outside the vocabulary, [2] bits of max|w_t·x_t|; then one group per
+// piece: 126 − min over its rows of ea (an atomicMax of a non-negative value).
+enum : int { WORD_COUNT = 0, WORD_BAD = 1, WORD_WX = 2, WORD_PIECES = 4 };
+
+// ------------------------------------------------------------------------------------------- labels
+
+// One workgroup lists the labelled rows in order: row_of[j] for j < count, place[r] = j or −1. A target of
+// LAYA_NO_LABEL carries no label; any other outside [0, vocab) is counted and carries none either.
+__global__ __launch_bounds__(1024) void label_rows_kernel(const int* __restrict__ targets, int rows, int vocab,
+                                                          int* __restrict__ row_of, int* __restrict__ place,
+                                                          unsigned* words, int n_words, int* bad_count, float* row_loss,
+                                                          float* lse) {
+    __shared__ int wave_count[16], wave_bad[16];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    int base = 0, bad = 0;
+    for (int r0 = 0; r0 < rows; r0 += 1024) {
+        const int r = r0 + tid;
+        const int y = r < rows ? targets[r] : LAYA_NO_LABEL;
+        const bool has = y >= 0 && y < vocab;
+        const unsigned long long m = __ballot(has);
+        const unsigned long long wrong = __ballot(!has && y != LAYA_NO_LABEL);
+        if (lane == 0) {
+            wave_count[wave] = __popcll(m);
+            wave_bad[wave] = __popcll(wrong);
+        }
+        __syncthreads();
+        int before = base;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) before += wave_count[w];
+            base += wave_count[w];
+            bad += wave_bad[w];
+        }
+        const int at = before + __popcll(m & ((1ull << lane) - 1));
+        if (has) row_of[at] = r;
+        if (r < rows) {
+            if (place) place[r] = has ? at : -1;
+            if (!has && row_loss) {
+                row_loss[r] = 0.0f;
+                lse[r] = 0.0f;
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < n_words; i += 1024) words[i] = i == WORD_COUNT ? base : i == WORD_BAD ? bad : 0;
+    if (tid == 0 && bad_count) *bad_count = bad;
+}
+
+// ------------------------------------------------------------------------------------------ packing
+
+// Eight consecutive values of a row from column c, zeros behind K. VEC: rows start on 16 bytes and K is a multiple of 8.
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* row, int c, int K, float (&v)[8]) {
+    if constexpr (VEC) {
+        const f32x4 zero = {};
+        const f32x4 a = c < K ? *reinterpret_cast<const f32x4*>(row + c) : zero;
+        const f32x4 b = c < K ? *reinterpret_cast<const f32x4*>(row + c + 4) : zero;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? row[c + i] : 0.0f;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v)[8]) {
+    if constexpr (VEC) {
+        const bf16x8 zero = {};
+        const bf16x8 a = c < K ? *reinterpret_cast<const bf16x8*>(row + c) : zero;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)row[c + i] : 0.0f;
+    }
+}
+
+struct PackRows {
+    const void* src;          // [.., K]
+    const int* row_of;        // source row of packed row j (null: j itself)
+    const unsigned* count;    // rows on the device (null: `rows`)
+    int rows, K;
+    int* exps;                // [rows padded to TILE]: the exponent of each row's scale
+    _Float16* out;            // rows as rows
+    _Float16* out_t;          // rows as k (null: not wanted)
+    int steps_t;
+    const float* bias;        // with `padded`: bias (or zeros) by row, −∞ behind the last
+    float* padded;
+    const float* weights;     // of the gathered source rows (null: 1), for `wx`
+    unsigned* wx;             // max |weight·x| as bits (null: not wanted)
+    unsigned* emin;           // 126 − min over the rows of exps (null: not wanted)
+};
+
+// One workgroup packs 32 rows, each scaled so that its largest finite magnitude lies in [2^14, 2^15): one read for the
+// magnitudes, one (from the caches) for the pieces. Thread t holds 8 columns of row t / 8. T: fp32 or bf16 source.
+template <typename T, int PLANES, bool VEC>
+__global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
+    constexpr int CHUNK = 64, PITCH = CHUNK + 1;
+    __shared__ unsigned turn[32 * PITCH];
+    __shared__ int row_exp[32];
+    const int b = blockIdx.x, tid = threadIdx.x, r = tid >> 3, o = tid & 7;
+    const int rows = p.count ? (int)*p.count : p.rows;
+    const int j = 32 * b + r;
+    if (32 * b >= rows) {  // behind the last block: what the tiles that reach over it read by row
+        if (o == 0 && p.padded && 32 * b < (p.rows + TILE - 1) / TILE * TILE) {
+            p.exps[j] = 0;
+            p.padded[j] = -__builtin_inff();
+        }
+        return;
+    }
+    const bool live = j < rows;
+    const int from = live ? (p.row_of ? p.row_of[j] : j) : 0;
+    const T* row = static_cast<const T*>(p.src) + (size_t)from * p.K;
+    unsigned am = 0;
+    if (live)
+        for (int c = o * 8; c < p.K; c += 64) {
+            float v[8];
+            load8<VEC>(row, c, p.K, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) am = max(am, amax_bits(v[i]));
+        }
+#pragma unroll
+    for (int s = 1; s < 8; s <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, s, 64));
+    const int e = pair_scale_exp(am);
+    if (o == 0) {
+        row_exp[r] = live ? e : 126;
+        if (p.exps) p.exps[j] = live ? e : 0;
+        if (p.padded) p.padded[j] = live ? (p.bias ? p.bias[j] : 0.0f) : -__builtin_inff();
+    }
+    if (p.wx) {
+        const float w = live && p.weights ? fabsf(p.weights[from]) : 1.0f;
+        unsigned m = live ? amax_bits(__builtin_bit_cast(float, am) * w) : 0u;
+#pragma unroll
+        for (int s = 8; s < 64; s <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, s, 64));
+        if ((tid & 63) == 0 && m) atomicMax(p.wx, m);
+    }
+    __syncthreads();
+    if (p.emin && tid < 32) {
+        int m = 126 - row_exp[tid];
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) m = max(m, __shfl_xor(m, s, 64));
+        if (tid == 0) atomicMax(p.emin, (unsigned)m);
+    }
+    const float sc = exp2_int(e);
+    const int steps = (p.K + 31) / 32 * 2, blocks_t = (p.K + 31) / 32;
+    for (int c0 = 0; c0 < p.K; c0 += CHUNK) {
+        float v[8];
+        const int c = c0 + o * 8, step = c >> 4;
+        if (live)
+            load8<VEC>(row, c, p.K, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        f16x8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            _Float16 h, l;
+            split_value(v[i] * sc, h, l);
+            hi[i] = h;
+            lo[i] = l;
+        }
+        if (step < steps) {
+            _Float16* at = p.out + ((size_t)b * steps + step) * (PLANES * FRAG) + ((o & 1) * 32 + r) * 8;
+            *reinterpret_cast<f16x8*>(at) = hi;
+            if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = lo;
+        }
+        if (p.out_t) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                turn[r * PITCH + o * 8 + i] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)hi[i]) |
+                                              (unsigned)__builtin_bit_cast(unsigned short, (_Float16)lo[i]) << 16;
+            __syncthreads();
+            const int h = tid & 63, u = tid >> 6;  // column c0 + h, rows 8u … 8u + 7
+            f16x8 th, tl;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned w = turn[(8 * u + i) * PITCH + h];
+                th[i] = __builtin_bit_cast(_Float16, (unsigned short)w);
+                tl[i] = __builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+            }
+            const int hb = (c0 + h) >> 5;
+            if (hb < blocks_t) {
+                _Float16* at = p.out_t + ((size_t)hb * p.steps_t + 2 * b + (u >> 1)) * (PLANES * FRAG) +
+                               ((u & 1) * 32 + (h & 31)) * 8;
+                *reinterpret_cast<f16x8*>(at) = th;
+                if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = tl;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// w_t·x_t of the labelled rows as an operand with rows h and k = t, one scale for all (from the word that pack_rows
+// left). One workgroup turns 32 rows x 64 columns. Rows without a label are not read, so that nothing in them counts.
+__global__ __launch_bounds__(256) void pack_weighted_kernel(const float* __restrict__ x, const float* __restrict__ weights,
+                                                            const int* __restrict__ row_of, const unsigned* words, int K,
+                                                            _Float16* __restrict__ out, int steps) {
+    constexpr int PITCH = 65;
+    __shared__ unsigned turn[32 * PITCH];
+    const int count = (int)words[WORD_COUNT], b = blockIdx.x, c0 = blockIdx.y * 64;
+    if (32 * b >= count) return;
+    const int tid = threadIdx.x, r = tid >> 3, o = tid & 7, j = 32 * b + r;
+    const float sc = exp2_int(pair_scale_exp(words[WORD_WX]));
+    float v[8] = {};
+    if (j < count) {
+        const int from = row_of[j];
+        load8<false>(x + (size_t)from * K, c0 + o * 8, K, v);
+        const float w = weights ? weights[from] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= w;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        _Float16 h, l;
+        split_value(v[i] * sc, h, l);
+        turn[r * PITCH + o * 8 + i] =
+            (unsigned)__builtin_bit_cast(unsigned short, h) | (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
+    }
+    __syncthreads();
+    const int h = tid & 63, u = tid >> 6, hb = (c0 + h) >> 5;
+    if (hb >= (K + 31) / 32) return;
+    f16x8 th, tl;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned w = turn[(8 * u + i) * PITCH + h];
+        th[i] = __builtin_bit_cast(_Float16, (unsigned short)w);
+        tl[i] = __builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+    }
+    _Float16* at = out + ((size_t)hb * steps + 2 * b + (u >> 1)) * (2 * FRAG) + ((u & 1) * 32 + (h & 31)) * 8;
+    *reinterpret_cast<f16x8*>(at) = th;
+    *reinterpret_cast<f16x8*>(at + FRAG) = tl;
+}
+
+// ------------------------------------------------------------------------------- logits and what they become
+
+struct Logits {
+    Operand W, x;              // W's piece: rows v; x: rows t
+    const int *ew, *ex;        // their rows' scale exponents
+    const float* bias;         // padded to whole tiles, −∞ behind the piece
+    const unsigned* words;
+    int v0, vocab;             // the piece's first row, its rows
+    int tiles_v;
+};
+
+// Tiles are taken in groups of 8 vocabulary tiles, all token tiles of a group before the next: 32 tiles in a row, what
+// an XCD runs at a time, share 8 of W's panels and 4 of x's.
+__device__ __forceinline__ void grouped_tile(int u, int tiles_v, int tiles_t, int& tv, int& tt) {
+    const int per = 8 * tiles_t, g = u / per, first = 8 * g, width = min(8, tiles_v - first), in = u - g * per;
+    tt = in / width;
+    tv = first + in - tt * width;
+}
+
+// The wave's logits from its accumulators, in place; `v` and `t`: the first of the wave's rows and columns.
+template <class Acc>
+__device__ __forceinline__ void to_logits(const Logits& p, Acc& acc, int v, int t, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = v + 32 * i + 8 * q + 4 * (lane >> 5);
+            const int4 ew = *reinterpret_cast<const int4*>(p.ew + at);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + at);
+            const int e[4] = {ew.x, ew.y, ew.z, ew.w};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int ex = p.ex[t + 32 * j + (lane & 31)];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    acc[i][j][4 * q + k] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + k], -(e[k] + ex)) + b[k];
+            }
+        }
+}
+
+// Each tile's maximum and Σ exp(z − maximum) for every row (token): part[tile_v][t].
+template <int PW>
+__global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* __restrict__ part, int pitch) {
+    typedef Tile<2, 4, 4, 2, PW, 2> T;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
+    const int count = (int)p.words[WORD_COUNT];
+    const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
+    p.x.blocks = (count + 31) / 32;
+    for (int n = 0;; ++n) {
+        const int u = unit_of(n);
+        if (n * (int)gridDim.x >= units) break;
+        if (u >= units) continue;
+        int tv, tt;
+        grouped_tile(u, p.tiles_v, tiles_t, tv, tt);
+        typename T::Acc acc;
+        T::product(p.W, p.x, tv * T::MB, tt * T::NB, 0, p.W.steps / 2, lds, acc, wave, lane);
+        to_logits(p, acc, tv * TILE + wm * 128, tt * TILE + wn * 64, lane);
+        float2* red = reinterpret_cast<float2*>(lds);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float m = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const float at = m == -__builtin_inff() ? 0.0f : m;
+            float s[4] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i] += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * LOG2E);
+            float sum = (s[0] + s[1]) + (s[2] + s[3]);
+            sum += __shfl_xor(sum, 32, 64);
+            if (lane < 32) red[wm * TILE + wn * 64 + 32 * j + lane] = make_float2(m, sum);
+        }
+        __syncthreads();
+        if (threadIdx.x < TILE) {
+            const float2 a = red[threadIdx.x], b = red[TILE + threadIdx.x];
+            const float m = fmaxf(a.x, b.x), at = m == -__builtin_inff() ? 0.0f : m;
+            const float sum = a.y * __builtin_amdgcn_exp2f((a.x - at) * LOG2E) +
+                              b.y * __builtin_amdgcn_exp2f((b.x - at) * LOG2E);
+            part[(size_t)(p.v0 / TILE + tv) * pitch + tt * TILE + threadIdx.x] = make_float2(m, sum);
+        }
+        __syncthreads();
+    }
+}
+
+// One wave a labelled row: the tiles' statistics merged, and the target's logit from W's row itself.
+template <typename TW>
+__global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restrict__ part, int pitch, int tiles,
+                                                          const unsigned* words, const int* __restrict__ row_of,
+                                                          const int* __restrict__ targets, const float* __restrict__ x,
+                                                          const TW* __restrict__ W, const float* __restrict__ bias,
+                                                          int hidden, float* __restrict__ row_loss,
+                                                          float* __restrict__ lse) {
+    const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (j >= (int)words[WORD_COUNT]) return;
+    const int r = row_of[j], y = targets[r];
+    float m = -__builtin_inff();
+    for (int k = lane; k < tiles; k += 64) m = fmaxf(m, part[(size_t)k * pitch + j].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    double s = 0.0, z = 0.0;
+    for (int k = lane; k < tiles; k += 64) {
+        const float2 a = part[(size_t)k * pitch + j];
+        if (a.y != 0.0f) s += (double)a.y * exp((double)a.x - (double)m);
+    }
+    for (int k = lane; k < hidden; k += 64) z += (double)x[(size_t)r * hidden + k] * (double)(float)W[(size_t)y * hidden + k];
+    s = wave_sum_d(s);
+    z = wave_sum_d(z);
+    if (lane == 0) {
+        const double l = (double)m + log(s);
+        lse[r] = (float)l;
+        row_loss[r] = (float)(l - (z + (bias ? (double)bias[y] : 0.0)));
+    }
+}
+
+// Σ w_r·loss_r·scale over the labelled rows, in a fixed order.
+__global__ __launch_bounds__(1024) void vocab_total_kernel(const float* __restrict__ row_loss, const unsigned* words,
+                                                           const int* __restrict__ row_of,
+                                                           const float* __restrict__ weights, float scale, float* loss) {
+    __shared__ double red[16];
+    const int count = (int)words[WORD_COUNT];
+    double s = 0.0;
+    for (int j = threadIdx.x; j < count; j += 1024) {
+        const int r = row_of[j];
+        s += (double)row_loss[r] * (weights ? (double)weights[r] : 1.0);
+    }
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) s += red[w];
+        *loss = (float)(s * (double)scale);
+    }
+}
+
+struct GradOut {
+    const int *row_of, *targets;
+    const float *lse, *weights;
+    const unsigned* emin;
+    _Float16* g;     // rows t, k = v: G·2^(G_SCALE + emin − ea[v])
+    _Float16* g_t;   // rows v, k = t: G·2^G_SCALE
+    int steps_v, steps_t, blocks_v;
+    float* db_part;  // [4 a token tile][padded piece] (null: no bias gradient)
+    int db_pitch;
+};
+
+// A piece's G in both orders.
+template <int PW, bool DB>
+__global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g) {
+    typedef Tile<2, 4, 4, 2, PW, 2> T;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
+    const int count = (int)p.words[WORD_COUNT];
+    const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
+    p.x.blocks = (count + 31) / 32;
+    const int emin = 126 - (int)*g.emin;
+    unsigned* turn = reinterpret_cast<unsigned*>(lds) + wave * (32 * TURN);
+    float* wl = reinterpret_cast<float*>(lds) + T::WAVES * 32 * TURN + wave * 64;
+    for (int n = 0;; ++n) {
+        const int u = unit_of(n);
+        if (n * (int)gridDim.x >= units) break;
+        if (u >= units) continue;
+        int tv, tt;
+        grouped_tile(u, p.tiles_v, tiles_t, tv, tt);
+        typename T::Acc acc;
+        T::product(p.W, p.x, tv * T::MB, tt * T::NB, 0, p.W.steps / 2, lds, acc, wave, lane);
+        const int v = tv * TILE + wm * 128, t = tt * TILE + wn * 64;
+        to_logits(p, acc, v, t, lane);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int at = t + 32 * j + (lane & 31);
+            const bool live = at < count;
+            const int r = live ? g.row_of[at] : 0;
+            const float lse = live ? g.lse[r] : 0.0f;
+            // The target's place among the lane's values: 32·i + 8·q + k of its first row's.
+            const int y = (live ? g.targets[r] : -1) - (p.v0 + v + 4 * (lane >> 5));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float x = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * LOG2E);
+                    x -= y == 32 * i + 8 * (e >> 2) + (e & 3) ? 1.0f : 0.0f;
+                    acc[i][j][e] = live ? x * (float)(1 << G_SCALE) : 0.0f;
+                }
+            if (DB && lane < 32) wl[32 * j + lane] = live ? (g.weights ? g.weights[r] : 1.0f) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int vb = (v >> 5) + i;
+            if (vb >= g.blocks_v) break;  // wave-uniform
+            float db = 0.0f;
+            int fold[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int4 ew = *reinterpret_cast<const int4*>(p.ew + v + 32 * i + 8 * q + 4 * (lane >> 5));
+                fold[4 * q] = emin - ew.x;
+                fold[4 * q + 1] = emin - ew.y;
+                fold[4 * q + 2] = emin - ew.z;
+                fold[4 * q + 3] = emin - ew.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int tb = (t >> 5) + j;
+                if (2 * tb >= g.steps_t) break;  // wave-uniform
+                f32x16 c = acc[i][j];
+                turn_write(c, turn, lane);
+#pragma unroll
+                for (int pass = 0; pass < 2; ++pass) {
+                    f16x8 hi, lo;
+                    turn_read(turn, lane, pass, hi, lo);
+                    _Float16* at = g.g_t + ((size_t)vb * g.steps_t + 2 * tb + pass) * (2 * FRAG) + lane * 8;
+                    *reinterpret_cast<f16x8*>(at) = hi;
+                    *reinterpret_cast<f16x8*>(at + FRAG) = lo;
+                    if constexpr (DB) {
+                        const float* w = wl + 32 * j + (2 * pass + (lane >> 5)) * 8;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) db = fmaf((float)hi[k] + (float)lo[k], w[k], db);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) c[e] = __builtin_amdgcn_ldexpf(c[e], fold[e]);
+                store_transposed(c, g.g + ((size_t)tb * g.steps_v + 2 * vb) * (2 * FRAG), lane);
+            }
+            if constexpr (DB) {
+                db += __shfl_xor(db, 32, 64);
+                if (lane < 32) g.db_part[(size_t)(tt * 4 + wn) * g.db_pitch + vb * 32 + lane] = db;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+struct GradProducts {
+    Operand g_t, wx;   // dW: rows v · rows h over t
+    Operand g, W_t;    // dx: rows t · rows h over v
+    const unsigned *words, *emin;
+    int vocab, hidden; // the piece's rows, the width
+    float* dW;         // the piece's first row
+    float scale;
+    float* dx_part;    // [split][padded rows][hidden]
+    int cap_rows;      // Σ over the splits of padded rows that dx_part holds (0: no dx)
+    int first;         // the first piece stores, the others add
+    int stages_first;  // the first piece's stages over v, which say how dx's sum is split
+    int tiles_v, tiles_h;
+};
+
+// The ways that dx's sum over a piece is split: so that its units are about as long as dW's, which run over the rows.
+__device__ __forceinline__ int dx_splits(int stages_v, int count, int cap_rows) {
+    const int padded = (count + TILE - 1) / TILE * TILE;
+    const int s = stages_v / max((count + 31) / 32, 96);
+    return max(1, min(min(s, MAX_SPLITS), cap_rows / max(padded, 1)));
+}
+
+// Both products of a piece in one launch.
+template <int PW>
+__global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) {
+    typedef Tile<2, 4, 4, 2, 2, 2> TE;
+    typedef Tile<2, 4, 4, 2, 2, PW> TX;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[TE::LDS_HALVES];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
+    const int count = (int)p.words[WORD_COUNT];
+    if (count == 0) return;
+    const int tiles_t = (count + TILE - 1) / TILE, stages_v = p.g.steps / 2;
+    const int splits = p.cap_rows ? dx_splits(p.stages_first, count, p.cap_rows) : 0;
+    const int units_e = p.tiles_v * p.tiles_h, units = units_e + tiles_t * p.tiles_h * splits;
+    const int e_wx = -(G_SCALE + pair_scale_exp(p.words[WORD_WX])), e_w = -(G_SCALE + 126 - (int)*p.emin);
+    p.g.blocks = (count + 31) / 32;
+    for (int n = 0;; ++n) {
+        const int u = unit_of(n);
+        if (n * (int)gridDim.x >= units) break;
+        if (u >= units) continue;
+        typename TE::Acc acc;
+        if (u < units_e) {
+            const int tv = u / p.tiles_h, th = u - tv * p.tiles_h;
+            TE::product(p.g_t, p.wx, tv * TE::MB, th * TE::NB, 0, (count + 31) / 32, lds, acc, wave, lane);
+            const int v = tv * TILE + wm * 128 + 4 * (lane >> 5), h = th * TILE + wn * 64 + (lane & 31);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (h + 32 * j >= p.hidden) continue;
+                    float old[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = v + 32 * i + 8 * (r >> 2) + (r & 3);
+                        old[r] = row < p.vocab ? p.dW[(size_t)row * p.hidden + h + 32 * j] : 0.0f;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = v + 32 * i + 8 * (r >> 2) + (r & 3);
+                        if (row < p.vocab)
+                            p.dW[(size_t)row * p.hidden + h + 32 * j] =
+                                old[r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_wx) * p.scale;
+                    }
+                }
+        } else {
+            const int w = u - units_e, per = tiles_t * p.tiles_h, s = w / per, in = w - s * per;
+            const int tt = in / p.tiles_h, th = in - tt * p.tiles_h;
+            const int s0 = (int)((long)stages_v * s / splits), s1 = (int)((long)stages_v * (s + 1) / splits);
+            TX::product(p.g, p.W_t, tt * TX::MB, th * TX::NB, s0, s1, lds, acc, wave, lane);
+            const int t = tt * TILE + wm * 128 + 4 * (lane >> 5), h = th * TILE + wn * 64 + (lane & 31);
+            float* out = p.dx_part + (size_t)s * tiles_t * TILE * p.hidden;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (h + 32 * j >= p.hidden) continue;
+                    float* at = out + (size_t)(t + 32 * i) * p.hidden + h + 32 * j;
+                    float old[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        old[r] = p.first ? 0.0f : at[(size_t)(8 * (r >> 2) + (r & 3)) * p.hidden];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        at[(size_t)(8 * (r >> 2) + (r & 3)) * p.hidden] =
+                            old[r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_w);
+                }
+        }
+    }
+}
+
+// dx_r = w_r·scale·Σ over the splits, 0 for rows without a label.
+__global__ __launch_bounds__(256) void vocab_dx_kernel(const float* __restrict__ part, const unsigned* words, int stages_v,
+                                                       int cap_rows, const int* __restrict__ place,
+                                                       const float* __restrict__ weights, float scale, int hidden,
+                                                       float* __restrict__ dx) {
+    const int r = blockIdx.x, j = place[r], count = (int)words[WORD_COUNT];
+    const int splits = dx_splits(stages_v, count, cap_rows);
+    const size_t stride = (size_t)((count + TILE - 1) / TILE * TILE) * hidden;
+    const float f = (weights ? weights[r] : 1.0f) * scale;
+    for (int h = threadIdx.x; h < hidden; h += 256) {
+        float s = 0.0f;
+        if (j >= 0) {
+            for (int k = 0; k < splits; ++k) s += part[k * stride + (size_t)j * hidden + h];
+            s *= f;
+        }
+        dx[(size_t)r * hidden + h] = s;
+    }
+}
+
+__global__ __launch_bounds__(256) void vocab_db_kernel(const float* __restrict__ part, int pitch, const unsigned* words,
+                                                       int vocab, float scale, float* __restrict__ db) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= vocab) return;
+    const int n = ((int)words[WORD_COUNT] + TILE - 1) / TILE * 4;
+    double s = 0.0;
+    for (int k = 0; k < n; ++k) s += part[(size_t)k * pitch + v];
+    db[v] += (float)(s * (double)scale * (1.0 / (1 << G_SCALE)));
+}
+
+// ------------------------------------------------------------------------------------------ launches
+
+long pad_tile(long n) { return (n + TILE - 1) / TILE * TILE; }
+
+template <typename T, int PLANES>
+void launch_pack(laya_ctx* ctx, const PackRows& p, int blocks) {
+    const bool vec = p.K % 8 == 0 && ((uintptr_t)p.src & 15u) == 0;
+    if (vec)
+        LAYA_LAUNCH((pack_rows_kernel<T, PLANES, true>), dim3(blocks), dim3(256), 0, ctx->stream, p);
+    else
+        LAYA_LAUNCH((pack_rows_kernel<T, PLANES, false>), dim3(blocks), dim3(256), 0, ctx->stream, p);
+    check_launch("pack_rows_kernel");
+}
+
+void pack_table(laya_ctx* ctx, const VocabArgs& a, int v0, int vocab, int* exps, float* padded, _Float16* out,
+                _Float16* out_t, unsigned* emin) {
+    PackRows p{};
+    p.src = a.W16 ? (const void*)(a.W16 + (size_t)v0 * a.hidden) : (const void*)(a.W + (size_t)v0 * a.hidden);
+    p.rows = vocab;
+    p.K = a.hidden;
+    p.exps = exps;
+    p.out = out;
+    p.out_t = out_t;
+    p.steps_t = k_steps(vocab);
+    p.bias = a.bias ? a.bias + v0 : nullptr;
+    p.padded = padded;
+    p.emin = emin;
+    const int blocks = (int)(pad_tile(vocab) / 32);
+    ProfileScope scope(ctx, "vocab_pack", 0.0, (a.W16 ? 2.0 : 4.0) * vocab * a.hidden * (out_t ? 3 : 2));
+    if (a.W16)
+        launch_pack<__bf16, 1>(ctx, p, blocks);
+    else
+        launch_pack<float, 2>(ctx, p, blocks);
+}
+
+void pack_states(laya_ctx* ctx, const VocabArgs& a, const int* row_of, unsigned* words, int* exps, _Float16* out,
+                 bool weighted) {
+    PackRows p{};
+    p.src = a.x;
+    p.row_of = row_of;
+    p.count = words + WORD_COUNT;
+    p.rows = a.rows;
+    p.K = a.hidden;
+    p.exps = exps;
+    p.out = out;
+    if (weighted) {
+        p.weights = a.row_weights;
+        p.wx = words + WORD_WX;
+    }
+    launch_pack<float, 2>(ctx, p, row_blocks(a.rows));
+}
+
+// Rows of the vocabulary a piece takes: whole tiles, pieces of about equal size, `each` bytes a row.
+int piece_rows(int vocab, size_t each) {
+    const long most = std::max<long>(TILE, (long)(PIECE_BYTES / each) / TILE * TILE);
+    const long pieces = (vocab + most - 1) / most;
+    return (int)std::min<long>(pad_tile((vocab + pieces - 1) / pieces), pad_tile(vocab));
+}
+
+int workgroups(const laya_ctx* ctx) { return std::max(8, ctx->cu_count / 8 * 8); }
+
+}  // namespace
+
+void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count) {
+    if (a.rows == 0) {
+        if (loss) fill(ctx, loss, 0.0f, 1);
+        if (bad_count) fill(ctx, reinterpret_cast<float*>(bad_count), 0.0f, 1);
+        return;
+    }
+    const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
+    const int piece = piece_rows(a.vocab, (size_t)k_steps(a.hidden) * 16 * 2 * planes);
+    const int tiles = (a.vocab + TILE - 1) / TILE;
+    unsigned* words;
+    int *row_of, *ex, *ew;
+    float* padded;
+    _Float16 *xp, *wp;
+    float2* part;
+    carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
+        ws.take(words, WORD_PIECES);
+        ws.take(row_of, a.rows);
+        ws.take(ex, pitch);
+        ws.take(ew, piece);
+        ws.take(padded, piece);
+        ws.take(xp, halves(a.rows, a.hidden, 2));
+        ws.take(wp, halves(piece, a.hidden, planes));
+        ws.take(part, (size_t)tiles * pitch);
+    });
+    LAYA_LAUNCH(label_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, a.targets, a.rows, a.vocab, row_of,
+                (int*)nullptr, words, (int)WORD_PIECES, bad_count, row_loss, lse);
+    check_launch("label_rows_kernel");
+    pack_states(ctx, a, row_of, words, ex, xp, false);
+    for (int v0 = 0; v0 < a.vocab; v0 += piece) {
+        const int n = std::min(piece, a.vocab - v0);
+        pack_table(ctx, a, v0, n, ew, padded, wp, nullptr, nullptr);
+        Logits p{{wp, k_steps(a.hidden), row_blocks(n)}, {xp, k_steps(a.hidden), 0}, ew, ex, padded, words, v0, n,
+                 (n + TILE - 1) / TILE};
+        ProfileScope scope(ctx, "vocab_stats", 2.0 * a.rows * a.hidden * n, 0.0);
+        if (a.W16)
+            LAYA_LAUNCH(vocab_stats_kernel<1>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, p, part, pitch);
+        else
+            LAYA_LAUNCH(vocab_stats_kernel<2>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, p, part, pitch);
+        check_launch("vocab_stats_kernel");
+    }
+    if (a.W16)
+        LAYA_LAUNCH(vocab_merge_kernel<__bf16>, dim3((a.rows + 3) / 4), dim3(256), 0, ctx->stream, part, pitch, tiles,
+                    words, row_of, a.targets, a.x, a.W16, a.bias, a.hidden, row_loss, lse);
+    else
+        LAYA_LAUNCH(vocab_merge_kernel<float>, dim3((a.rows + 3) / 4), dim3(256), 0, ctx->stream, part, pitch, tiles,
+                    words, row_of, a.targets, a.x, a.W, a.bias, a.hidden, row_loss, lse);
+    check_launch("vocab_merge_kernel");
+    if (loss) {
+        LAYA_LAUNCH(vocab_total_kernel, dim3(1), dim3(1024), 0, ctx->stream, row_loss, words, row_of, a.row_weights,
+                    a.scale, loss);
+        check_launch("vocab_total_kernel");
+    }
+}
+
+void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {
+    if (a.rows == 0) return;
+    const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = k_steps(a.hidden);
+    const int steps_t = k_steps(a.rows);
+    const int piece =
+        piece_rows(a.vocab, (size_t)steps_h * 16 * 4 * planes + (size_t)steps_t * 16 * 8);
+    const int pieces = (a.vocab + piece - 1) / piece, n_words = WORD_PIECES + pieces;
+    const int cap_rows = std::max(pitch, std::min(MAX_SPLITS * pitch, 32768));
+    const int tiles_t = pitch / TILE, tiles_h = (a.hidden + TILE - 1) / TILE;
+    unsigned* words;
+    int *row_of, *place, *ex, *ew;
+    float *padded, *part, *db_part;
+    _Float16 *xp, *xt, *wp, *wt, *gp, *gt;
+    carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
+        ws.take(words, n_words);
+        ws.take(row_of, a.rows);
+        ws.take(place, a.rows);
+        ws.take(ex, pitch);
+        ws.take(ew, piece);
+        ws.take(padded, piece);
+        ws.take(xp, halves(a.rows, a.hidden, 2));
+        ws.take(xt, halves(a.hidden, a.rows, 2));
+        ws.take(wp, halves(piece, a.hidden, planes));
+        ws.take(wt, dx ? halves(a.hidden, piece, planes) : 0);
+        ws.take(gp, halves(a.rows, piece, 2));
+        ws.take(gt, halves(piece, a.rows, 2));
+        ws.take(part, dx ? (size_t)cap_rows * a.hidden : 0);
+        ws.take(db_part, db ? (size_t)tiles_t * 4 * piece : 0);
+    });
+    if (!db) db_part = nullptr;
+    LAYA_LAUNCH(label_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, a.targets, a.rows, a.vocab, row_of, place, words,
+                n_words, (int*)nullptr, (float*)nullptr, (float*)nullptr);
+    check_launch("label_rows_kernel");
+    pack_states(ctx, a, row_of, words, ex, xp, true);
+    LAYA_LAUNCH(pack_weighted_kernel, dim3(row_blocks(a.rows), (a.hidden + 63) / 64), dim3(256), 0, ctx->stream, a.x,
+                a.row_weights, row_of, words, a.hidden, xt, steps_t);
+    check_launch("pack_weighted_kernel");
+    int stages_v = 0;
+    for (int v0 = 0, k = 0; v0 < a.vocab; v0 += piece, ++k) {
+        const int n = std::min(piece, a.vocab - v0), tiles_v = (n + TILE - 1) / TILE;
+        // Every piece splits dx's sum as the first does, so that its partial sums meet the first's.
+        if (v0 == 0) stages_v = k_steps(n) / 2;
+        unsigned* emin = words + WORD_PIECES + k;
+        pack_table(ctx, a, v0, n, ew, padded, wp, dx ? wt : nullptr, emin);
+        Logits p{{wp, steps_h, row_blocks(n)}, {xp, steps_h, 0}, ew, ex, padded, words, v0, n, tiles_v};
+        GradOut g{row_of, a.targets, lse, a.row_weights, emin, gp, gt, k_steps(n), steps_t, row_blocks(n), db_part,
+                  piece};
+        {
+            ProfileScope scope(ctx, "vocab_grad", 2.0 * a.rows * a.hidden * n, 0.0);
+            const dim3 grid(workgroups(ctx)), block(512);
+            if (a.W16 && db)
+                LAYA_LAUNCH((vocab_grad_kernel<1, true>), grid, block, 0, ctx->stream, p, g);
+            else if (a.W16)
+                LAYA_LAUNCH((vocab_grad_kernel<1, false>), grid, block, 0, ctx->stream, p, g);
+            else if (db)
+                LAYA_LAUNCH((vocab_grad_kernel<2, true>), grid, block, 0, ctx->stream, p, g);
+            else
+                LAYA_LAUNCH((vocab_grad_kernel<2, false>), grid, block, 0, ctx->stream, p, g);
+            check_launch("vocab_grad_kernel");
+        }
+        GradProducts q{};
+        q.g_t = {gt, steps_t, row_blocks(n)};
+        q.wx = {xt, steps_t, row_blocks(a.hidden)};
+        q.g = {gp, k_steps(n), 0};
+        q.W_t = {wt, k_steps(n), row_blocks(a.hidden)};
+        q.words = words;
+        q.emin = emin;
+        q.vocab = n;
+        q.hidden = a.hidden;
+        q.dW = dW ? dW + (size_t)v0 * a.hidden : nullptr;
+        q.scale = a.scale;
+        q.dx_part = part;
+        q.cap_rows = dx ? cap_rows : 0;
+        q.first = v0 == 0;
+        q.stages_first = stages_v;
+        q.tiles_v = dW ? tiles_v : 0;
+        q.tiles_h = tiles_h;
+        if (dx || dW) {
+            ProfileScope scope(ctx, "vocab_products", ((dx ? 2.0 : 0.0) + (dW ? 2.0 : 0.0)) * a.rows * a.hidden * n, 0.0);
+            if (a.W16)
+                LAYA_LAUNCH(vocab_products_kernel<1>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, q);
+            else
+                LAYA_LAUNCH(vocab_products_kernel<2>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, q);
+            check_launch("vocab_products_kernel");
+        }
+        if (db) {
+            LAYA_LAUNCH(vocab_db_kernel, dim3((n + 255) / 256), dim3(256), 0, ctx->stream, db_part, piece, words, n,
+                        a.scale, db + v0);
+            check_launch("vocab_db_kernel");
+        }
+    }
+    if (dx) {
+        LAYA_LAUNCH(vocab_dx_kernel, dim3(a.rows), dim3(256), 0, ctx->stream, part, words, stages_v, cap_rows, place,
+                    a.row_weights, a.scale, a.hidden, dx);
+        check_launch("vocab_dx_kernel");
+    }
+}
+
+}  // namespace laya

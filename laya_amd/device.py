@@ -88,7 +88,7 @@ class Context:
 
 
 class DeviceArray:
-    """A device allocation with a shape and dtype (fp32 or int32)."""
+    """A device allocation with a shape and dtype (fp32 or int32; uint16 for bf16 bit patterns)."""
 
     def __init__(self, ctx: Context, shape: Sequence[int], dtype=np.float32, zero: bool = True):
         self.ctx = ctx
@@ -111,6 +111,22 @@ class DeviceArray:
         d.upload(a)
         return d
 
+    @classmethod
+    def borrow(cls, ctx: Context, ptr: int, shape: Sequence[int], dtype=np.float32, owner=None) -> "DeviceArray":
+        """Contiguous device memory that something else owns (a torch tensor's, a part of an arena) as an array; `owner`
+        is kept alive, free() leaves the memory alone. Calls run on the context's stream: work on other streams that
+        writes or reads the memory is ordered by the caller."""
+        d = cls.__new__(cls)
+        d.ctx = ctx
+        d.shape = tuple(int(s) for s in shape)
+        d.dtype = np.dtype(dtype)
+        d.size = int(np.prod(d.shape)) if d.shape else 1
+        d.nbytes = d.size * d.dtype.itemsize
+        d.ptr = int(ptr) if ptr else None
+        d.owner = owner
+        d.borrowed = True
+        return d
+
     def upload(self, a: np.ndarray) -> None:
         a = np.ascontiguousarray(a, dtype=self.dtype)
         assert a.size == self.size, f"size {a.size} vs {self.size}"
@@ -126,9 +142,10 @@ class DeviceArray:
         check(lib().laya_fill(self.ctx.handle, self.ptr, float(value), self.size))
 
     def free(self) -> None:
-        if getattr(self, "ptr", None) and getattr(self.ctx, "handle", None):
+        if not getattr(self, "borrowed", False) and getattr(self, "ptr", None) and getattr(self.ctx, "handle", None):
             lib().laya_free(self.ctx.handle, self.ptr)
         self.ptr = None
+        self.owner = None
 
     def __del__(self):
         try:

@@ -28,6 +28,15 @@ class Parameter:
         self.trainable = trainable
         self._grad: Optional[DeviceArray] = None
 
+    @classmethod
+    def borrow(cls, ctx: Context, name: str, shape: Sequence[int], data: Optional[DeviceArray],
+               gradient: Optional[DeviceArray] = None, trainable: bool = True) -> "Parameter":
+        """A parameter over arrays that are there already (DeviceArray.borrow's, or an arena's)."""
+        p = cls.__new__(cls)
+        p.ctx, p.name, p.shape = ctx, name, tuple(int(n) for n in shape)
+        p.data, p.trainable, p._grad = data, trainable, gradient
+        return p
+
     @property
     def gradient(self) -> Optional[DeviceArray]:
         return self._grad
@@ -357,6 +366,52 @@ def softmax_ce_backward(ctx: Context, logits: DeviceArray, targets: DeviceArray,
                         loss: Optional[DeviceArray] = None) -> None:
     check(lib().laya_softmax_ce_bwd(_h(ctx), logits.ptr, targets.ptr, option_offsets.ptr, n_items, ce_weight, scale,
                                     grad.ptr, ptr(loss)))
+
+
+NO_LABEL = -100  # a target without a label (laya_hip.h: LAYA_NO_LABEL)
+
+
+def _vocab_args(weight: Parameter, bias: Optional[Parameter], x: DeviceArray, targets: DeviceArray, rows: int,
+                row_weights: Optional[DeviceArray], scale: float, weight16: Optional[DeviceArray]) -> tuple:
+    vocab, hidden = weight.shape
+    if rows < 0 or x.size < rows * hidden or targets.size < rows:
+        raise ValueError(f"vocab_ce: x {x.shape} and targets {targets.shape} for {rows} rows of width {hidden}")
+    if targets.dtype != np.int32:
+        raise ValueError(f"vocab_ce: targets are int32, not {targets.dtype}")
+    if row_weights is not None and row_weights.size < rows:
+        raise ValueError(f"vocab_ce: {row_weights.size} row weights for {rows} rows")
+    if bias is not None and bias.shape != (vocab,):
+        raise ValueError(f"vocab_ce: bias {bias.shape} for {vocab} vocabulary entries")
+    if weight16 is not None and weight16.size != vocab * hidden:
+        raise ValueError(f"vocab_ce: bf16 weight of {weight16.size} values for {vocab} x {hidden}")
+    return (_h(weight.ctx), x.ptr, rows, hidden, None if weight16 is not None else weight.data.ptr, ptr(weight16), vocab,
+            None if bias is None else bias.data.ptr, targets.ptr, ptr(row_weights), scale)
+
+
+def vocab_ce(weight: Parameter, bias: Optional[Parameter], x: DeviceArray, targets: DeviceArray, rows: int,
+             row_loss: DeviceArray, lse: DeviceArray, row_weights: Optional[DeviceArray] = None, scale: float = 1.0,
+             loss: Optional[DeviceArray] = None, weight16: Optional[DeviceArray] = None,
+             bad_count: Optional[DeviceArray] = None) -> None:
+    """Softmax cross entropy of x's rows over the vocabulary, the logits x·Wᵀ + b never held: row_loss and lse by row,
+    loss = scale·Σ row_weights·row_loss. Rows whose target is NO_LABEL cost and count nothing. weight16: the weight as
+    bf16 bit patterns (a uint16 array), read instead of its fp32 values (laya_vocab_ce_fwd)."""
+    args = _vocab_args(weight, bias, x, targets, rows, row_weights, scale, weight16)
+    if row_loss.size < rows or lse.size < rows:
+        raise ValueError(f"vocab_ce: row_loss {row_loss.shape} and lse {lse.shape} for {rows} rows")
+    check(lib().laya_vocab_ce_fwd(*args, row_loss.ptr, lse.ptr, ptr(loss), ptr(bad_count)))
+
+
+def vocab_ce_backward(weight: Parameter, bias: Optional[Parameter], x: DeviceArray, targets: DeviceArray, rows: int,
+                      lse: DeviceArray, dx: Optional[DeviceArray], row_weights: Optional[DeviceArray] = None,
+                      scale: float = 1.0, weight16: Optional[DeviceArray] = None) -> None:
+    """vocab_ce's backward from its lse: dx is overwritten (as linear_backward's), the weight's and the bias's gradients
+    accumulate (laya_vocab_ce_bwd)."""
+    args = _vocab_args(weight, bias, x, targets, rows, row_weights, scale, weight16)
+    if lse.size < rows or (dx is not None and dx.size < rows * weight.shape[1]):
+        raise ValueError(f"vocab_ce_backward: lse {lse.shape} and dx for {rows} rows of width {weight.shape[1]}")
+    dW = weight.gradient_buffer().ptr if weight.trainable else None
+    db = bias.gradient_buffer().ptr if (bias is not None and bias.trainable) else None
+    check(lib().laya_vocab_ce_bwd(*args, lse.ptr, ptr(dx), dW, db))
 
 
 def rlcd_objective(ctx: Context, logits: DeviceArray, targets: DeviceArray, option_offsets: DeviceArray,
