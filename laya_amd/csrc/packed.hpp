@@ -4,183 +4,235 @@
 // An fp32 operand that several tiles read is split once into the fp16 pieces of split2h_4 (a power-of-two scale, then
 // hi + lo, 22 bits) and kept in the order in which the matrix cores take it, so that the product's loop converts
 // nothing and computes no addresses: it copies runs of memory to LDS (16 bytes a lane, no registers between) and reads
-// fragments back, both linear. v_mfma_f32_32x32x16_f16 takes from lane l the 8 k of half l / 32 of row l mod 32, so a
-// fragment is 32 rows x 16 k = 1 KB, [half][row][8 k], and an operand of R rows and K columns is
-//   [⌈R / 32⌉ row blocks][k steps][planes: hi, lo][512 fp16]
-// with zeros behind R and K, the number of k steps even (the loop takes two to a stage). bf16-valued operands keep one
-// plane (split1h_4). Three piece products make one fp32-accurate product (lo·hi, hi·lo, hi·hi), two when one side has
-// one plane.
+// fragments back, both linear. v_mfma_f32_16x16x32_f16 takes from lane l the 8 k of l / 16 of row l mod 16, so a
+// fragment is 16 rows x 32 k = 1 KB, [k / 8][row][8 k], and an operand of R rows and K columns is
+//   [⌈R / 32⌉ row groups][⌈K / 32⌉ steps][2 halves of 16 rows][planes: hi, lo][512 fp16]
+// with zeros behind R and K. bf16-valued operands keep one plane (split1h_4). Three piece products make one
+// fp32-accurate product (lo·hi, hi·lo, hi·hi), two when one side has one plane.
+//
+// These products are bound by the power that the matrix cores draw, not by their rate: on random fp16 data (registers
+// and LDS alone) 16x16x32 reaches 1.81 PFLOP/s and 32x32x16 1.59, on zeros both 2.38. Hence the 16 x 16 form.
 #pragma once
+#include <type_traits>
+
 #include "common.hpp"
 #include "split.hpp"
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 namespace laya {
 namespace packed {
 
 constexpr int FRAG = 512;  // fp16 values of a fragment
 
-inline int row_blocks(long rows) { return (int)((rows + 31) / 32); }
-inline int k_steps(long k) { return (int)((k + 31) / 32) * 2; }  // 16-deep, even
-inline size_t halves(long rows, long k, int planes) { return (size_t)row_blocks(rows) * k_steps(k) * planes * FRAG; }
+inline int groups_of(long rows) { return (int)((rows + 31) / 32); }
+inline int steps_of(long k) { return (int)((k + 31) / 32); }
+inline size_t halves(long rows, long k, int planes) { return (size_t)groups_of(rows) * steps_of(k) * 2 * planes * FRAG; }
 
-// A packed operand as a kernel takes it. `blocks`: its row blocks (a tile's blocks behind the last read the last).
+// A packed operand as a kernel takes it. `groups`: its row groups (a tile's groups behind the last read the last).
 struct Operand {
     const _Float16* data;
-    int steps, blocks;
+    int steps, groups;
 };
+
+// Where the hi plane's 8 values of row r, columns 8·o …, of a row group's step start (o: the octet of the 32 columns).
+template <int PLANES>
+__device__ __forceinline__ int unit_at(int r, int o) {
+    return ((r >> 4) * PLANES * 4 + o) * 128 + (r & 15) * 8;
+}
 
 __device__ __forceinline__ void split_value(float v, _Float16& hi, _Float16& lo) {
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);
 }
 
-// 16 bytes a lane from global memory to LDS, the wave's 64 lanes in a row from `to` (the same in every lane).
-template <int OFFSET>
-__device__ __forceinline__ void copy_to_lds(const _Float16* from, _Float16* to) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                     (__attribute__((address_space(3))) void*)to, 16, OFFSET, 0);
+// KB KB from global memory to LDS, 16 bytes a lane and KB, the wave's 64 lanes in a row from LDS byte `to` (the same in
+// every lane). Written as assembly, which takes no register for the data: around the builtin the compiler lets every
+// LDS read wait for all reads before it (it cannot tell the copy's target from theirs), and the loop's look-ahead is
+// lost. The loop waits for the copies itself (wait_copies).
+template <int KB>
+__device__ __forceinline__ void copy_to_lds(const _Float16* from, unsigned to) {
+    static_assert(KB == 2 || KB == 4, "a row group's step");
+    if constexpr (KB == 4)
+        asm volatile(
+            "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+            "global_load_lds_dwordx4 %1, off offset:1024\n\tglobal_load_lds_dwordx4 %1, off offset:2048\n\t"
+            "global_load_lds_dwordx4 %1, off offset:3072" ::"s"(to), "v"(from) : "memory");
+    else
+        asm volatile(
+            "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+            "global_load_lds_dwordx4 %1, off offset:1024" ::"s"(to), "v"(from) : "memory");
+}
+// Waits for the wave's copies (and its other memory accesses), then for the whole workgroup: what every wave copied is
+// in LDS, and every wave's reads before this point are done.
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_byte(const void* p) {
+    return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-// A workgroup of WAVES_M x WAVES_N waves, each BM x BN blocks of 32 x 32 outputs: C[m, n] += Σ_k A[m, k]·B[n, k].
+// A workgroup of WAVES_M x WAVES_N waves, each BM x BN blocks of 16 x 16 outputs: C[m, n] += Σ_k A[m, k]·B[n, k].
+//
+// LDS holds two 32-deep steps. A step's barrier stands before its last row block's products: by then every wave has read
+// the step to the end and the next step's copies, started a step ago, have landed; behind it the copies of the step
+// after that start into the buffer just read, and the next step's first fragments are read while the last products run.
+// Between two barriers a wave has a whole step's products, and no read or copy is waited for where it is issued.
 template <int WAVES_M, int WAVES_N, int BM, int BN, int PA, int PB>
 struct Tile {
     static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
-    static constexpr int MB = WAVES_M * BM, NB = WAVES_N * BN;  // row blocks of A and B in a tile
-    static constexpr int M = 32 * MB, N = 32 * NB;
-    static constexpr int A_HALVES = MB * 2 * PA * FRAG, STAGE = A_HALVES + NB * 2 * PB * FRAG;
-    static constexpr int LDS_HALVES = 2 * STAGE;
-    static_assert((MB + NB) % WAVES == 0, "every wave copies the same number of blocks");
-    static constexpr int COPIES = (MB + NB) / WAVES;
+    static constexpr int M = WAVES_M * BM * 16, N = WAVES_N * BN * 16;
+    static constexpr int MG = M / 32, NG = N / 32;  // row groups of A and B in a tile
+    static constexpr int A_HALVES = MG * 2 * PA * FRAG, STEP = A_HALVES + NG * 2 * PB * FRAG;
+    static constexpr int LDS_HALVES = 2 * STEP;
+    static constexpr int PER_WAVE = (MG + NG) / WAVES;  // row groups a wave copies each step
+    static_assert((MG + NG) % WAVES == 0 && PER_WAVE <= 2 && (PA == PB || MG % WAVES == 0) && BM % 2 == 0, "tile shape");
 
-    typedef f32x16 Acc[BM][BN];
+    typedef f32x4 Acc[BM][BN];
 
-    // Stage st (two 16-deep steps) into LDS: block b of A, then of B, each 2·planes KB.
-    static __device__ __forceinline__ void load(const Operand& a, const Operand& b, int mb0, int nb0, int st,
-                                                _Float16* stage, int wave, int lane) {
-#pragma unroll
-        for (int c = 0; c < COPIES; ++c) {
-            const int i = wave + c * WAVES;  // wave-uniform
-            if (i < MB) {
-                const _Float16* g = a.data +
-                                    ((size_t)min(mb0 + i, a.blocks - 1) * a.steps + 2 * st) * (PA * FRAG) + lane * 8;
-                _Float16* l = stage + i * (2 * PA * FRAG);
-                copy_to_lds<0>(g, l);
-                copy_to_lds<1024>(g, l);
-                if constexpr (PA == 2) {
-                    copy_to_lds<2048>(g, l);
-                    copy_to_lds<3072>(g, l);
-                }
-            } else {
-                const _Float16* g = b.data + ((size_t)min(nb0 + i - MB, b.blocks - 1) * b.steps + 2 * st) * (PB * FRAG) +
-                                    lane * 8;
-                _Float16* l = stage + A_HALVES + (i - MB) * (2 * PB * FRAG);
-                copy_to_lds<0>(g, l);
-                copy_to_lds<1024>(g, l);
-                if constexpr (PB == 2) {
-                    copy_to_lds<2048>(g, l);
-                    copy_to_lds<3072>(g, l);
-                }
-            }
+    // Planes of the c-th row group that a wave copies (A's come first).
+    static constexpr int planes(int c) { return MG % WAVES == 0 ? (c < MG / WAVES ? PA : PB) : PA; }
+
+    struct Copies {
+        const _Float16* from[PER_WAVE];
+        unsigned to[PER_WAVE];
+        // Starts a step's copies into the buffer at byte `slot`, and moves on to the next step.
+        __device__ __forceinline__ void start(unsigned slot) {
+            copy<0>(slot);
+            if constexpr (PER_WAVE > 1) copy<1>(slot);
         }
+        template <int C>
+        __device__ __forceinline__ void copy(unsigned slot) {
+            copy_to_lds<2 * planes(C)>(from[C], to[C] + slot);
+            from[C] += 2 * planes(C) * FRAG;
+        }
+    };
+
+    static __device__ __forceinline__ void read_a(const _Float16* step, int i, f16x8 (&a)[PA]) {
+#pragma unroll
+        for (int p = 0; p < PA; ++p) a[p] = *reinterpret_cast<const f16x8*>(step + (i * PA + p) * FRAG);
+    }
+    static __device__ __forceinline__ void read_b(const _Float16* step, int j, f16x8 (&b)[PB]) {
+#pragma unroll
+        for (int p = 0; p < PB; ++p) b[p] = *reinterpret_cast<const f16x8*>(step + (j * PB + p) * FRAG);
+    }
+    // The pieces' products, smallest first: of a whole row block, piece by piece (no product waits for the one before),
+    // and of one block.
+    static __device__ __forceinline__ void mma(const f16x8 (&a)[PA], const f16x8 (&b)[BN][PB], f32x4 (&c)[BN]) {
+        if constexpr (PA == 2)
+#pragma unroll
+            for (int j = 0; j < BN; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], b[j][0], c[j], 0, 0, 0);
+        if constexpr (PB == 2)
+#pragma unroll
+            for (int j = 0; j < BN; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[j][1], c[j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[j][0], c[j], 0, 0, 0);
+    }
+    static __device__ __forceinline__ void mma1(const f16x8 (&a)[PA], const f16x8 (&b)[PB], f32x4& c) {
+        if constexpr (PA == 2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], b[0], c, 0, 0, 0);
+        if constexpr (PB == 2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[0], c, 0, 0, 0);
     }
 
-    // One stage: B's fragments of a step once, A's a row block ahead. The scheduling barriers keep each group's reads
-    // ahead of the products before it; left alone the compiler sinks them to their use, and every block waits for LDS.
-    static __device__ __forceinline__ void multiply(const _Float16* stage, Acc& acc, int wm, int wn, int lane) {
-        const _Float16* as = stage + wm * BM * (2 * PA * FRAG) + lane * 8;
-        const _Float16* bs = stage + A_HALVES + wn * BN * (2 * PB * FRAG) + lane * 8;
-        f16x8 a[2][PA], b[2][BN][PB];
-        auto read_a = [&](int g) {
-#pragma unroll
-            for (int p = 0; p < PA; ++p)
-                a[g & 1][p] = *reinterpret_cast<const f16x8*>(as + (((g % BM) * 2 + g / BM) * PA + p) * FRAG);
-        };
-        auto read_b = [&](int s) {
-#pragma unroll
-            for (int j = 0; j < BN; ++j)
-#pragma unroll
-                for (int p = 0; p < PB; ++p)
-                    b[s][j][p] = *reinterpret_cast<const f16x8*>(bs + ((j * 2 + s) * PB + p) * FRAG);
-        };
-        read_b(0);
-        read_a(0);
-#pragma unroll
-        for (int g = 0; g < 2 * BM; ++g) {
-            const int s = g / BM, i = g % BM;
-            if (g + 1 < 2 * BM) read_a(g + 1);
-            if (g == (BM > 1 ? BM - 2 : 0)) read_b(1);
-            __builtin_amdgcn_sched_barrier(0);
-            // The pieces' products, smallest first.
-#pragma unroll
-            for (int j = 0; j < BN; ++j)
-                if constexpr (PA == 2)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[g & 1][1], b[s][j][0], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < BN; ++j)
-                if constexpr (PB == 2)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[g & 1][0], b[s][j][1], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int j = 0; j < BN; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[g & 1][0], b[s][j][0], acc[i][j], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-
-    // acc = Σ over stages [s0, s1) of the tile at row blocks mb0 of A and nb0 of B. Every thread of the workgroup calls
-    // it with the same arguments; it ends with the LDS free.
-    static __device__ __forceinline__ void product(const Operand& a, const Operand& b, int mb0, int nb0, int s0, int s1,
+    // acc = Σ over steps [s0, s1) of the tile at row groups mg0 of A and ng0 of B. Every thread of the workgroup calls it
+    // with the same arguments; it ends with the LDS free.
+    static __device__ __forceinline__ void product(const Operand& a, const Operand& b, int mg0, int ng0, int s0, int s1,
                                                    _Float16* lds, Acc& acc, int wave, int lane) {
         const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 #pragma unroll
         for (int i = 0; i < BM; ++i)
 #pragma unroll
-            for (int j = 0; j < BN; ++j) acc[i][j] = f32x16{};
-        if (s0 < s1) load(a, b, mb0, nb0, s0, lds, wave, lane);
-        for (int st = s0; st < s1; ++st) {
-            const int cur = (st - s0) & 1;
-            // The stage's copies have landed, and every wave is done with the other buffer.
-            __builtin_amdgcn_s_waitcnt(0);
-            __builtin_amdgcn_s_barrier();
-            if (st + 1 < s1) load(a, b, mb0, nb0, st + 1, lds + (cur ^ 1) * STAGE, wave, lane);
-            multiply(lds + cur * STAGE, acc, wm, wn, lane);
+            for (int j = 0; j < BN; ++j) acc[i][j] = f32x4{};
+        if (s0 >= s1) return;
+        Copies cp;
+        const unsigned lds0 = lds_byte(lds);
+#pragma unroll
+        for (int c = 0; c < PER_WAVE; ++c) {
+            const int i = __builtin_amdgcn_readfirstlane(wave + c * WAVES);
+            cp.from[c] =
+                i < MG ? a.data + ((size_t)min(mg0 + i, a.groups - 1) * a.steps + s0) * (2 * PA * FRAG) + lane * 8
+                       : b.data + ((size_t)min(ng0 + i - MG, b.groups - 1) * b.steps + s0) * (2 * PB * FRAG) + lane * 8;
+            cp.to[c] = lds0 + 2 * (i < MG ? i * (2 * PA * FRAG) : A_HALVES + (i - MG) * (2 * PB * FRAG));
         }
+        const _Float16* as = lds + wm * BM * (PA * FRAG) + lane * 8;
+        const _Float16* bs = lds + A_HALVES + wn * BN * (PB * FRAG) + lane * 8;
+        cp.start(0);
+        wait_copies();
+        if (s1 - s0 > 1) cp.start(2 * STEP);
+        f16x8 fa[2][PA], fb[BN][PB];
+        read_a(as, 0, fa[0]);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) read_b(bs, j, fb[j]);
+        // One step from buffer H (its fragments of B in fb, A's first in fa[0]); the last row block's products hand fb over
+        // to the next step's, block by block. What is read ahead of the last step's end is of a buffer that no one needs.
+        auto step = [&](auto buffer, bool more) {
+            constexpr int H = decltype(buffer)::value;
+            const _Float16 *at = as + H * STEP, *an = as + (H ^ 1) * STEP, *bn = bs + (H ^ 1) * STEP;
+#pragma unroll
+            for (int i = 0; i + 1 < BM; ++i) {
+                read_a(at, i + 1, fa[(i + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(fa[i & 1], fb, acc[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            wait_copies();
+            if (more) cp.start(H * (2 * STEP));
+            read_a(an, 0, fa[0]);
+#pragma unroll
+            for (int j = 0; j < BN; ++j) {
+                mma1(fa[1], fb[j], acc[BM - 1][j]);
+                __builtin_amdgcn_sched_barrier(0);
+                read_b(bn, j, fb[j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        const std::integral_constant<int, 0> first;
+        const std::integral_constant<int, 1> second;
+        int s = s0;
+        for (; s + 1 < s1; s += 2) {
+            step(first, s + 2 < s1);
+            step(second, s + 3 < s1);
+        }
+        if (s < s1) step(first, false);
         __syncthreads();
     }
 };
 
-// A 32 x 32 block of outputs C[m, n] in one wave's accumulator: lane l holds column n = l mod 32, rows
-// m = 8·(r / 4) + 4·(l / 32) + r mod 4. Written as fragments of Cᵀ (rows n, k = m): eight bytes a lane, each pair of
-// lanes l, l + 32 filling a row's 16. `to`: the fragment pair's address for row block n / 32 and step m / 16.
-__device__ __forceinline__ void store_transposed(const f32x16& c, _Float16* to, int lane) {
+// 32 x 32 outputs C[m, n] as two by two blocks of one wave's accumulator: lane l holds column n = l mod 16 of a block,
+// rows m = 4·(l / 16) … + 3.
+
+// Written as a row group's step of Cᵀ (rows n, k = m), eight bytes a lane.
+__device__ __forceinline__ void store_transposed(const f32x4 (&c)[2][2], _Float16* to, int lane) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        f16x4 hi, lo;
-        split2h_4(f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]}, 1.0f, hi, lo);
-        _Float16* at = to + (q >> 1) * (2 * FRAG) + ((q & 1) * 32 + (lane & 31)) * 8 + 4 * (lane >> 5);
-        *reinterpret_cast<f16x4*>(at) = hi;
-        *reinterpret_cast<f16x4*>(at + FRAG) = lo;
-    }
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            f16x4 hi, lo;
+            split2h_4(c[i][j], 1.0f, hi, lo);
+            _Float16* at = to + unit_at<2>(16 * j + (lane & 15), 2 * i + (lane >> 5)) + 4 * ((lane >> 4) & 1);
+            *reinterpret_cast<f16x4*>(at) = hi;
+            *reinterpret_cast<f16x4*>(at + FRAG) = lo;
+        }
 }
 
-// The same block as fragments of C (rows m, k = n), turned in LDS: 32 rows of TURN dwords of the wave's own, each value
-// as its two pieces in a dword. Rows 4 apart lie 32 banks apart (the two halves of a wave write without a conflict),
-// and 8 consecutive rows' 16 bytes lie in different banks.
-constexpr int TURN = 40, TURN_HALVES = 32 * TURN * 2;
-__device__ __forceinline__ void turn_write(const f32x16& c, unsigned* turn, int lane) {
+// The same outputs turned in LDS to a row group's step of C (rows m, k = n): 32 rows of TURN dwords of the wave's own,
+// each value as its two pieces in a dword. The rows that a write's four quarters meet lie 16 banks apart, and 16
+// consecutive rows' 16 bytes in different banks.
+constexpr int TURN = 36, TURN_DWORDS = 32 * TURN;
+__device__ __forceinline__ void turn_write(const f32x4 (&c)[2][2], unsigned* turn, int lane) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        _Float16 hi, lo;
-        split_value(c[r], hi, lo);
-        turn[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * TURN + (lane & 31)] =
-            (unsigned)__builtin_bit_cast(unsigned short, hi) | (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
-    }
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                _Float16 hi, lo;
+                split_value(c[i][j][r], hi, lo);
+                turn[(16 * i + 4 * (lane >> 4) + r) * TURN + 16 * j + (lane & 15)] =
+                    (unsigned)__builtin_bit_cast(unsigned short, hi) |
+                    (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
+            }
 }
-// Unit (row lane mod 32, columns 8·o … 8·o + 7) of the turned block, o = 2·pass + lane / 32.
-__device__ __forceinline__ void turn_read(const unsigned* turn, int lane, int pass, f16x8& hi, f16x8& lo) {
+// The lane's unit of row half i: row 16·i + l mod 16, columns 8·(l / 16) … + 7.
+__device__ __forceinline__ void turn_read(const unsigned* turn, int lane, int i, f16x8& hi, f16x8& lo) {
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const unsigned* at = turn + (lane & 31) * TURN + (2 * pass + (lane >> 5)) * 8;
+    const unsigned* at = turn + (16 * i + (lane & 15)) * TURN + (lane >> 4) * 8;
     const u32x4 x = *reinterpret_cast<const u32x4*>(at), y = *reinterpret_cast<const u32x4*>(at + 4);
     u32x4 h, l;
     h[0] = __builtin_amdgcn_perm(x[1], x[0], 0x05040100u);

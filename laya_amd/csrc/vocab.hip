@@ -22,12 +22,12 @@ using namespace packed;
 constexpr int TILE = 256;            // logits, G and both gradient products run on 256 x 256 tiles
 constexpr int G_SCALE = 14;          // |G| ≤ 1
 constexpr int MAX_SPLITS = 16;       // ways of dx's sum over a piece of the vocabulary
-constexpr size_t PIECE_BYTES = (size_t)2 << 30;  // of packed table and G that a piece of the vocabulary may take
+constexpr size_t PIECE_BYTES = (size_t)3 << 30;  // of packed table and G that a piece of the vocabulary may take
 constexpr float LOG2E = 1.44269504088896341f;
 
-// Words of a call: [0] labelled rows, [1] targets outside the vocabulary, [2] bits of max|w_t·x_t|; then one group per
-// piece: 126 − min over its rows of ea (an atomicMax of a non-negative value).
-enum : int { WORD_COUNT = 0, WORD_BAD = 1, WORD_WX = 2, WORD_PIECES = 4 };
+// Words of a call: [0] labelled rows, [1] targets outside the vocabulary, [2] bits of max|w_t·x_t|,
+// [3] the ways dx's sum is split; then a word a piece: 126 − min over its rows of ea (an atomicMax of a non-negative value).
+enum : int { WORD_COUNT = 0, WORD_BAD = 1, WORD_WX = 2, WORD_SPLITS = 3, WORD_PIECES = 4 };
 
 // ------------------------------------------------------------------------------------------- labels
 
@@ -172,10 +172,10 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
         if (tid == 0) atomicMax(p.emin, (unsigned)m);
     }
     const float sc = exp2_int(e);
-    const int steps = (p.K + 31) / 32 * 2, blocks_t = (p.K + 31) / 32;
+    const int steps = (p.K + 31) / 32;
     for (int c0 = 0; c0 < p.K; c0 += CHUNK) {
         float v[8];
-        const int c = c0 + o * 8, step = c >> 4;
+        const int c = c0 + o * 8, step = c >> 5;
         if (live)
             load8<VEC>(row, c, p.K, v);
         else
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
             lo[i] = l;
         }
         if (step < steps) {
-            _Float16* at = p.out + ((size_t)b * steps + step) * (PLANES * FRAG) + ((o & 1) * 32 + r) * 8;
+            _Float16* at = p.out + ((size_t)b * steps + step) * (2 * PLANES * FRAG) + unit_at<PLANES>(r, o & 3);
             *reinterpret_cast<f16x8*>(at) = hi;
             if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = lo;
         }
@@ -208,10 +208,9 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
                 th[i] = __builtin_bit_cast(_Float16, (unsigned short)w);
                 tl[i] = __builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
             }
-            const int hb = (c0 + h) >> 5;
-            if (hb < blocks_t) {
-                _Float16* at = p.out_t + ((size_t)hb * p.steps_t + 2 * b + (u >> 1)) * (PLANES * FRAG) +
-                               ((u & 1) * 32 + (h & 31)) * 8;
+            const int hg = (c0 + h) >> 5;
+            if (hg < steps) {
+                _Float16* at = p.out_t + ((size_t)hg * p.steps_t + b) * (2 * PLANES * FRAG) + unit_at<PLANES>(h & 31, u);
                 *reinterpret_cast<f16x8*>(at) = th;
                 if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = tl;
             }
@@ -247,8 +246,8 @@ __global__ __launch_bounds__(256) void pack_weighted_kernel(const float* __restr
             (unsigned)__builtin_bit_cast(unsigned short, h) | (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
     }
     __syncthreads();
-    const int h = tid & 63, u = tid >> 6, hb = (c0 + h) >> 5;
-    if (hb >= (K + 31) / 32) return;
+    const int h = tid & 63, u = tid >> 6, hg = (c0 + h) >> 5;
+    if (hg >= (K + 31) / 32) return;
     f16x8 th, tl;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -256,7 +255,7 @@ __global__ __launch_bounds__(256) void pack_weighted_kernel(const float* __restr
         th[i] = __builtin_bit_cast(_Float16, (unsigned short)w);
         tl[i] = __builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
     }
-    _Float16* at = out + ((size_t)hb * steps + 2 * b + (u >> 1)) * (2 * FRAG) + ((u & 1) * 32 + (h & 31)) * 8;
+    _Float16* at = out + ((size_t)hg * steps + b) * (4 * FRAG) + unit_at<2>(h & 31, u);
     *reinterpret_cast<f16x8*>(at) = th;
     *reinterpret_cast<f16x8*>(at + FRAG) = tl;
 }
@@ -283,33 +282,31 @@ __device__ __forceinline__ void grouped_tile(int u, int tiles_v, int tiles_t, in
 // The wave's logits from its accumulators, in place; `v` and `t`: the first of the wave's rows and columns.
 template <class Acc>
 __device__ __forceinline__ void to_logits(const Logits& p, Acc& acc, int v, int t, int lane) {
+    int ex[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) ex[j] = p.ex[t + 16 * j + (lane & 15)];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int at = v + 32 * i + 8 * q + 4 * (lane >> 5);
-            const int4 ew = *reinterpret_cast<const int4*>(p.ew + at);
-            const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + at);
-            const int e[4] = {ew.x, ew.y, ew.z, ew.w};
+    for (int i = 0; i < 8; ++i) {
+        const int at = v + 16 * i + 4 * (lane >> 4);
+        const int4 ew = *reinterpret_cast<const int4*>(p.ew + at);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + at);
+        const int e[4] = {ew.x, ew.y, ew.z, ew.w};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int ex = p.ex[t + 32 * j + (lane & 31)];
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    acc[i][j][4 * q + k] = __builtin_amdgcn_ldexpf(acc[i][j][4 * q + k], -(e[k] + ex)) + b[k];
-            }
-        }
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_ldexpf(acc[i][j][r], -(e[r] + ex[j])) + b[r];
+    }
 }
 
 // Each tile's maximum and Σ exp(z − maximum) for every row (token): part[tile_v][t].
 template <int PW>
 __global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* __restrict__ part, int pitch) {
-    typedef Tile<2, 4, 4, 2, PW, 2> T;
+    typedef Tile<2, 4, 8, 4, PW, 2> T;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
     const int count = (int)p.words[WORD_COUNT];
     const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
-    p.x.blocks = (count + 31) / 32;
+    p.x.groups = (count + 31) / 32;
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
@@ -317,26 +314,28 @@ __global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* _
         int tv, tt;
         grouped_tile(u, p.tiles_v, tiles_t, tv, tt);
         typename T::Acc acc;
-        T::product(p.W, p.x, tv * T::MB, tt * T::NB, 0, p.W.steps / 2, lds, acc, wave, lane);
+        T::product(p.W, p.x, tv * T::MG, tt * T::NG, 0, p.W.steps, lds, acc, wave, lane);
         to_logits(p, acc, tv * TILE + wm * 128, tt * TILE + wn * 64, lane);
         float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < 4; ++j) {
             float m = -__builtin_inff();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+                for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const float at = m == -__builtin_inff() ? 0.0f : m;
             float s[4] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[i] += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * LOG2E);
+                for (int r = 0; r < 4; ++r) s[r] += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * LOG2E);
             float sum = (s[0] + s[1]) + (s[2] + s[3]);
+            sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
-            if (lane < 32) red[wm * TILE + wn * 64 + 32 * j + lane] = make_float2(m, sum);
+            if (lane < 16) red[wm * TILE + wn * 64 + 16 * j + lane] = make_float2(m, sum);
         }
         __syncthreads();
         if (threadIdx.x < TILE) {
@@ -406,7 +405,7 @@ struct GradOut {
     const unsigned* emin;
     _Float16* g;     // rows t, k = v: G·2^(G_SCALE + emin − ea[v])
     _Float16* g_t;   // rows v, k = t: G·2^G_SCALE
-    int steps_v, steps_t, blocks_v;
+    int steps_v, steps_t, groups_v;
     float* db_part;  // [4 a token tile][padded piece] (null: no bias gradient)
     int db_pitch;
 };
@@ -414,15 +413,15 @@ struct GradOut {
 // A piece's G in both orders.
 template <int PW, bool DB>
 __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g) {
-    typedef Tile<2, 4, 4, 2, PW, 2> T;
+    typedef Tile<2, 4, 8, 4, PW, 2> T;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
     const int count = (int)p.words[WORD_COUNT];
     const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
-    p.x.blocks = (count + 31) / 32;
+    p.x.groups = (count + 31) / 32;
     const int emin = 126 - (int)*g.emin;
-    unsigned* turn = reinterpret_cast<unsigned*>(lds) + wave * (32 * TURN);
-    float* wl = reinterpret_cast<float*>(lds) + T::WAVES * 32 * TURN + wave * 64;
+    unsigned* turn = reinterpret_cast<unsigned*>(lds) + wave * TURN_DWORDS;
+    float* wl = reinterpret_cast<float*>(lds) + T::WAVES * TURN_DWORDS + wave * 64;
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
@@ -430,67 +429,79 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
         int tv, tt;
         grouped_tile(u, p.tiles_v, tiles_t, tv, tt);
         typename T::Acc acc;
-        T::product(p.W, p.x, tv * T::MB, tt * T::NB, 0, p.W.steps / 2, lds, acc, wave, lane);
+        T::product(p.W, p.x, tv * T::MG, tt * T::NG, 0, p.W.steps, lds, acc, wave, lane);
         const int v = tv * TILE + wm * 128, t = tt * TILE + wn * 64;
         to_logits(p, acc, v, t, lane);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int at = t + 32 * j + (lane & 31);
+        for (int j = 0; j < 4; ++j) {
+            const int at = t + 16 * j + (lane & 15);
             const bool live = at < count;
             const int r = live ? g.row_of[at] : 0;
             const float lse = live ? g.lse[r] : 0.0f;
-            // The target's place among the lane's values: 32·i + 8·q + k of its first row's.
-            const int y = (live ? g.targets[r] : -1) - (p.v0 + v + 4 * (lane >> 5));
+            // The target's place among the lane's values: 16·i + e.
+            const int y = (live ? g.targets[r] : -1) - (p.v0 + v + 4 * (lane >> 4));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
+                for (int e = 0; e < 4; ++e) {
                     float x = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * LOG2E);
-                    x -= y == 32 * i + 8 * (e >> 2) + (e & 3) ? 1.0f : 0.0f;
+                    x -= y == 16 * i + e ? 1.0f : 0.0f;
                     acc[i][j][e] = live ? x * (float)(1 << G_SCALE) : 0.0f;
                 }
-            if (DB && lane < 32) wl[32 * j + lane] = live ? (g.weights ? g.weights[r] : 1.0f) : 0.0f;
+            if (DB && lane < 16) wl[16 * j + lane] = live ? (g.weights ? g.weights[r] : 1.0f) : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int vb = (v >> 5) + i;
-            if (vb >= g.blocks_v) break;  // wave-uniform
-            float db = 0.0f;
-            int fold[16];
+            const int vg = (v >> 5) + i;
+            if (vg >= g.groups_v) break;  // wave-uniform
+            float db[2] = {0.0f, 0.0f};
+            int fold[2][4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int4 ew = *reinterpret_cast<const int4*>(p.ew + v + 32 * i + 8 * q + 4 * (lane >> 5));
-                fold[4 * q] = emin - ew.x;
-                fold[4 * q + 1] = emin - ew.y;
-                fold[4 * q + 2] = emin - ew.z;
-                fold[4 * q + 3] = emin - ew.w;
+            for (int q = 0; q < 2; ++q) {
+                const int4 ew = *reinterpret_cast<const int4*>(p.ew + v + 32 * i + 16 * q + 4 * (lane >> 4));
+                fold[q][0] = emin - ew.x;
+                fold[q][1] = emin - ew.y;
+                fold[q][2] = emin - ew.z;
+                fold[q][3] = emin - ew.w;
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int tb = (t >> 5) + j;
-                if (2 * tb >= g.steps_t) break;  // wave-uniform
-                f32x16 c = acc[i][j];
+                const int tg = (t >> 5) + j;
+                if (tg >= g.steps_t) break;  // wave-uniform
+                f32x4 c[2][2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) c[q][k] = acc[2 * i + q][2 * j + k];
                 turn_write(c, turn, lane);
+                _Float16* at = g.g_t + ((size_t)vg * g.steps_t + tg) * (4 * FRAG) + lane * 8;
 #pragma unroll
-                for (int pass = 0; pass < 2; ++pass) {
+                for (int q = 0; q < 2; ++q) {
                     f16x8 hi, lo;
-                    turn_read(turn, lane, pass, hi, lo);
-                    _Float16* at = g.g_t + ((size_t)vb * g.steps_t + 2 * tb + pass) * (2 * FRAG) + lane * 8;
-                    *reinterpret_cast<f16x8*>(at) = hi;
-                    *reinterpret_cast<f16x8*>(at + FRAG) = lo;
+                    turn_read(turn, lane, q, hi, lo);
+                    *reinterpret_cast<f16x8*>(at + 2 * q * FRAG) = hi;
+                    *reinterpret_cast<f16x8*>(at + (2 * q + 1) * FRAG) = lo;
                     if constexpr (DB) {
-                        const float* w = wl + 32 * j + (2 * pass + (lane >> 5)) * 8;
+                        const float* w = wl + 32 * j + (lane >> 4) * 8;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) db = fmaf((float)hi[k] + (float)lo[k], w[k], db);
+                        for (int k = 0; k < 8; ++k) db[q] = fmaf((float)hi[k] + (float)lo[k], w[k], db[q]);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) c[e] = __builtin_amdgcn_ldexpf(c[e], fold[e]);
-                store_transposed(c, g.g + ((size_t)tb * g.steps_v + 2 * vb) * (2 * FRAG), lane);
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[q][k][e] = __builtin_amdgcn_ldexpf(c[q][k][e], fold[q][e]);
+                store_transposed(c, g.g + ((size_t)tg * g.steps_v + vg) * (4 * FRAG), lane);
             }
             if constexpr (DB) {
-                db += __shfl_xor(db, 32, 64);
-                if (lane < 32) g.db_part[(size_t)(tt * 4 + wn) * g.db_pitch + vb * 32 + lane] = db;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    db[q] += __shfl_xor(db[q], 16, 64);
+                    db[q] += __shfl_xor(db[q], 32, 64);
+                    if (lane < 16) g.db_part[(size_t)(tt * 4 + wn) * g.db_pitch + vg * 32 + 16 * q + lane] = db[q];
+                }
             }
         }
         __syncthreads();
@@ -500,38 +511,56 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
 struct GradProducts {
     Operand g_t, wx;   // dW: rows v · rows h over t
     Operand g, W_t;    // dx: rows t · rows h over v
-    const unsigned *words, *emin;
+    unsigned* words;
+    const unsigned* emin;
     int vocab, hidden; // the piece's rows, the width
     float* dW;         // the piece's first row
     float scale;
     float* dx_part;    // [split][padded rows][hidden]
     int cap_rows;      // Σ over the splits of padded rows that dx_part holds (0: no dx)
     int first;         // the first piece stores, the others add
-    int stages_first;  // the first piece's stages over v, which say how dx's sum is split
+    int steps_first, units_first;  // the first piece's steps over v and units of dW, which say how dx's sum is split
     int tiles_v, tiles_h;
 };
 
-// The ways that dx's sum over a piece is split: so that its units are about as long as dW's, which run over the rows.
-__device__ __forceinline__ int dx_splits(int stages_v, int count, int cap_rows) {
-    const int padded = (count + TILE - 1) / TILE * TILE;
-    const int s = stages_v / max((count + 31) / 32, 96);
-    return max(1, min(min(s, MAX_SPLITS), cap_rows / max(padded, 1)));
+// The ways that dx's sum over a piece is split: those of 1 … MAX_SPLITS whose longest worker ends first. Worker w of G
+// takes units w, w + G, …: dW's ne (each `le` steps), then dx's; the longest is the first of a class of equals.
+__device__ __forceinline__ int dx_splits(int steps_v, int count, int cap_rows, int ne, int tiles_h, int G) {
+    const int tiles_t = (count + TILE - 1) / TILE, le = (count + 31) / 32;
+    const int most = max(1, min(min(MAX_SPLITS, steps_v), cap_rows / max(tiles_t * TILE, 1)));
+    int best = 1;
+    long best_time = 1l << 60;
+    for (int s = 1; s <= most; ++s) {
+        const int units = ne + tiles_t * tiles_h * s, lx = (steps_v + s - 1) / s;
+        long time = 0;
+        for (int w = 0; w < G; w = w == 0 && ne % G != 0 ? ne % G : G) {
+            const int mine = (units - w + G - 1) / G, e = max(0, (ne - w + G - 1) / G);
+            // Each unit costs about 24 steps beside its own: the first copies, the stores.
+            time = max(time, (long)e * (le + 24) + (long)(mine - e) * (lx + 24));
+        }
+        if (time < best_time) {
+            best_time = time;
+            best = s;
+        }
+    }
+    return best;
 }
 
 // Both products of a piece in one launch.
 template <int PW>
 __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) {
-    typedef Tile<2, 4, 4, 2, 2, 2> TE;
-    typedef Tile<2, 4, 4, 2, 2, PW> TX;
+    typedef Tile<2, 4, 8, 4, 2, 2> TE;
+    typedef Tile<2, 4, 8, 4, 2, PW> TX;
     __shared__ __attribute__((aligned(16))) _Float16 lds[TE::LDS_HALVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
     const int count = (int)p.words[WORD_COUNT];
     if (count == 0) return;
-    const int tiles_t = (count + TILE - 1) / TILE, stages_v = p.g.steps / 2;
-    const int splits = p.cap_rows ? dx_splits(p.stages_first, count, p.cap_rows) : 0;
+    const int tiles_t = (count + TILE - 1) / TILE, steps_v = p.g.steps;
+    const int splits = p.cap_rows ? dx_splits(p.steps_first, count, p.cap_rows, p.units_first, p.tiles_h, gridDim.x) : 0;
     const int units_e = p.tiles_v * p.tiles_h, units = units_e + tiles_t * p.tiles_h * splits;
     const int e_wx = -(G_SCALE + pair_scale_exp(p.words[WORD_WX])), e_w = -(G_SCALE + 126 - (int)*p.emin);
-    p.g.blocks = (count + 31) / 32;
+    p.g.groups = (count + 31) / 32;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.words[WORD_SPLITS] = splits;
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
@@ -539,60 +568,61 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
         typename TE::Acc acc;
         if (u < units_e) {
             const int tv = u / p.tiles_h, th = u - tv * p.tiles_h;
-            TE::product(p.g_t, p.wx, tv * TE::MB, th * TE::NB, 0, (count + 31) / 32, lds, acc, wave, lane);
-            const int v = tv * TILE + wm * 128 + 4 * (lane >> 5), h = th * TILE + wn * 64 + (lane & 31);
+            TE::product(p.g_t, p.wx, tv * TE::MG, th * TE::NG, 0, (count + 31) / 32, lds, acc, wave, lane);
+            const int v = tv * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i) {
+                float old[4][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (h + 32 * j >= p.hidden) continue;
-                    float old[16];
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = v + 32 * i + 8 * (r >> 2) + (r & 3);
-                        old[r] = row < p.vocab ? p.dW[(size_t)row * p.hidden + h + 32 * j] : 0.0f;
+                    for (int r = 0; r < 4; ++r) {
+                        const bool in = h + 16 * j < p.hidden && v + 16 * i + r < p.vocab;
+                        old[j][r] = in ? p.dW[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] : 0.0f;
                     }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = v + 32 * i + 8 * (r >> 2) + (r & 3);
-                        if (row < p.vocab)
-                            p.dW[(size_t)row * p.hidden + h + 32 * j] =
-                                old[r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_wx) * p.scale;
-                    }
-                }
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (h + 16 * j < p.hidden && v + 16 * i + r < p.vocab)
+                            p.dW[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] =
+                                old[j][r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_wx) * p.scale;
+            }
         } else {
             const int w = u - units_e, per = tiles_t * p.tiles_h, s = w / per, in = w - s * per;
             const int tt = in / p.tiles_h, th = in - tt * p.tiles_h;
-            const int s0 = (int)((long)stages_v * s / splits), s1 = (int)((long)stages_v * (s + 1) / splits);
-            TX::product(p.g, p.W_t, tt * TX::MB, th * TX::NB, s0, s1, lds, acc, wave, lane);
-            const int t = tt * TILE + wm * 128 + 4 * (lane >> 5), h = th * TILE + wn * 64 + (lane & 31);
+            const int s0 = (int)((long)steps_v * s / splits), s1 = (int)((long)steps_v * (s + 1) / splits);
+            TX::product(p.g, p.W_t, tt * TX::MG, th * TX::NG, s0, s1, lds, acc, wave, lane);
+            const int t = tt * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
             float* out = p.dx_part + (size_t)s * tiles_t * TILE * p.hidden;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 8; ++i) {
+                float old[4][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (h + 32 * j >= p.hidden) continue;
-                    float* at = out + (size_t)(t + 32 * i) * p.hidden + h + 32 * j;
-                    float old[16];
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        old[r] = p.first ? 0.0f : at[(size_t)(8 * (r >> 2) + (r & 3)) * p.hidden];
+                    for (int r = 0; r < 4; ++r)
+                        old[j][r] = !p.first && h + 16 * j < p.hidden
+                                        ? out[(size_t)(t + 16 * i + r) * p.hidden + h + 16 * j]
+                                        : 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        at[(size_t)(8 * (r >> 2) + (r & 3)) * p.hidden] =
-                            old[r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_w);
-                }
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (h + 16 * j < p.hidden)
+                            out[(size_t)(t + 16 * i + r) * p.hidden + h + 16 * j] =
+                                old[j][r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_w);
+            }
         }
     }
 }
 
 // dx_r = w_r·scale·Σ over the splits, 0 for rows without a label.
-__global__ __launch_bounds__(256) void vocab_dx_kernel(const float* __restrict__ part, const unsigned* words, int stages_v,
-                                                       int cap_rows, const int* __restrict__ place,
+__global__ __launch_bounds__(256) void vocab_dx_kernel(const float* __restrict__ part, const unsigned* words,
+                                                       const int* __restrict__ place,
                                                        const float* __restrict__ weights, float scale, int hidden,
                                                        float* __restrict__ dx) {
-    const int r = blockIdx.x, j = place[r], count = (int)words[WORD_COUNT];
-    const int splits = dx_splits(stages_v, count, cap_rows);
+    const int r = blockIdx.x, j = place[r], count = (int)words[WORD_COUNT], splits = (int)words[WORD_SPLITS];
     const size_t stride = (size_t)((count + TILE - 1) / TILE * TILE) * hidden;
     const float f = (weights ? weights[r] : 1.0f) * scale;
     for (int h = threadIdx.x; h < hidden; h += 256) {
@@ -638,7 +668,7 @@ void pack_table(laya_ctx* ctx, const VocabArgs& a, int v0, int vocab, int* exps,
     p.exps = exps;
     p.out = out;
     p.out_t = out_t;
-    p.steps_t = k_steps(vocab);
+    p.steps_t = steps_of(vocab);
     p.bias = a.bias ? a.bias + v0 : nullptr;
     p.padded = padded;
     p.emin = emin;
@@ -664,7 +694,7 @@ void pack_states(laya_ctx* ctx, const VocabArgs& a, const int* row_of, unsigned*
         p.weights = a.row_weights;
         p.wx = words + WORD_WX;
     }
-    launch_pack<float, 2>(ctx, p, row_blocks(a.rows));
+    launch_pack<float, 2>(ctx, p, groups_of(a.rows));
 }
 
 // Rows of the vocabulary a piece takes: whole tiles, pieces of about equal size, `each` bytes a row.
@@ -685,7 +715,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
         return;
     }
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
-    const int piece = piece_rows(a.vocab, (size_t)k_steps(a.hidden) * 16 * 2 * planes);
+    const int piece = piece_rows(a.vocab, (size_t)steps_of(a.hidden) * 32 * 2 * planes);
     const int tiles = (a.vocab + TILE - 1) / TILE;
     unsigned* words;
     int *row_of, *ex, *ew;
@@ -709,7 +739,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
     for (int v0 = 0; v0 < a.vocab; v0 += piece) {
         const int n = std::min(piece, a.vocab - v0);
         pack_table(ctx, a, v0, n, ew, padded, wp, nullptr, nullptr);
-        Logits p{{wp, k_steps(a.hidden), row_blocks(n)}, {xp, k_steps(a.hidden), 0}, ew, ex, padded, words, v0, n,
+        Logits p{{wp, steps_of(a.hidden), groups_of(n)}, {xp, steps_of(a.hidden), 0}, ew, ex, padded, words, v0, n,
                  (n + TILE - 1) / TILE};
         ProfileScope scope(ctx, "vocab_stats", 2.0 * a.rows * a.hidden * n, 0.0);
         if (a.W16)
@@ -734,10 +764,10 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
 
 void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {
     if (a.rows == 0) return;
-    const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = k_steps(a.hidden);
-    const int steps_t = k_steps(a.rows);
+    const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = steps_of(a.hidden);
+    const int steps_t = steps_of(a.rows);
     const int piece =
-        piece_rows(a.vocab, (size_t)steps_h * 16 * 4 * planes + (size_t)steps_t * 16 * 8);
+        piece_rows(a.vocab, (size_t)steps_h * 32 * 4 * planes + (size_t)steps_t * 32 * 8);
     const int pieces = (a.vocab + piece - 1) / piece, n_words = WORD_PIECES + pieces;
     const int cap_rows = std::max(pitch, std::min(MAX_SPLITS * pitch, 32768));
     const int tiles_t = pitch / TILE, tiles_h = (a.hidden + TILE - 1) / TILE;
@@ -766,18 +796,21 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
                 n_words, (int*)nullptr, (float*)nullptr, (float*)nullptr);
     check_launch("label_rows_kernel");
     pack_states(ctx, a, row_of, words, ex, xp, true);
-    LAYA_LAUNCH(pack_weighted_kernel, dim3(row_blocks(a.rows), (a.hidden + 63) / 64), dim3(256), 0, ctx->stream, a.x,
+    LAYA_LAUNCH(pack_weighted_kernel, dim3(groups_of(a.rows), (a.hidden + 63) / 64), dim3(256), 0, ctx->stream, a.x,
                 a.row_weights, row_of, words, a.hidden, xt, steps_t);
     check_launch("pack_weighted_kernel");
-    int stages_v = 0;
+    int steps_v = 0, units_e = 0;
     for (int v0 = 0, k = 0; v0 < a.vocab; v0 += piece, ++k) {
         const int n = std::min(piece, a.vocab - v0), tiles_v = (n + TILE - 1) / TILE;
         // Every piece splits dx's sum as the first does, so that its partial sums meet the first's.
-        if (v0 == 0) stages_v = k_steps(n) / 2;
+        if (v0 == 0) {
+            steps_v = steps_of(n);
+            units_e = dW ? tiles_v * tiles_h : 0;
+        }
         unsigned* emin = words + WORD_PIECES + k;
         pack_table(ctx, a, v0, n, ew, padded, wp, dx ? wt : nullptr, emin);
-        Logits p{{wp, steps_h, row_blocks(n)}, {xp, steps_h, 0}, ew, ex, padded, words, v0, n, tiles_v};
-        GradOut g{row_of, a.targets, lse, a.row_weights, emin, gp, gt, k_steps(n), steps_t, row_blocks(n), db_part,
+        Logits p{{wp, steps_h, groups_of(n)}, {xp, steps_h, 0}, ew, ex, padded, words, v0, n, tiles_v};
+        GradOut g{row_of, a.targets, lse, a.row_weights, emin, gp, gt, steps_of(n), steps_t, groups_of(n), db_part,
                   piece};
         {
             ProfileScope scope(ctx, "vocab_grad", 2.0 * a.rows * a.hidden * n, 0.0);
@@ -793,10 +826,10 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
             check_launch("vocab_grad_kernel");
         }
         GradProducts q{};
-        q.g_t = {gt, steps_t, row_blocks(n)};
-        q.wx = {xt, steps_t, row_blocks(a.hidden)};
-        q.g = {gp, k_steps(n), 0};
-        q.W_t = {wt, k_steps(n), row_blocks(a.hidden)};
+        q.g_t = {gt, steps_t, groups_of(n)};
+        q.wx = {xt, steps_t, groups_of(a.hidden)};
+        q.g = {gp, steps_of(n), 0};
+        q.W_t = {wt, steps_of(n), groups_of(a.hidden)};
         q.words = words;
         q.emin = emin;
         q.vocab = n;
@@ -806,7 +839,8 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
         q.dx_part = part;
         q.cap_rows = dx ? cap_rows : 0;
         q.first = v0 == 0;
-        q.stages_first = stages_v;
+        q.steps_first = steps_v;
+        q.units_first = units_e;
         q.tiles_v = dW ? tiles_v : 0;
         q.tiles_h = tiles_h;
         if (dx || dW) {
@@ -824,8 +858,7 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
         }
     }
     if (dx) {
-        LAYA_LAUNCH(vocab_dx_kernel, dim3(a.rows), dim3(256), 0, ctx->stream, part, words, stages_v, cap_rows, place,
-                    a.row_weights, a.scale, a.hidden, dx);
+        LAYA_LAUNCH(vocab_dx_kernel, dim3(a.rows), dim3(256), 0, ctx->stream, part, words, place, a.row_weights, a.scale, a.hidden, dx);
         check_launch("vocab_dx_kernel");
     }
 }
