@@ -10,6 +10,11 @@
 // with zeros behind R and K. bf16-valued operands keep one plane (split1h_4). Three piece products make one
 // fp32-accurate product (lo·hi, hi·lo, hi·hi), two when one side has one plane.
 //
+// The same memory serves a product over the operand's rows (its columns then being the product's rows): a row group's
+// step is 32 x 32 values either way, and ds_read_b64_tr_b16 hands each lane four rows of its column. Octet o's rows
+// stand rotated by 4·o, so that the four rows x two octets that such a read meets lie in different banks; a linear read
+// takes each lane's unit through the same rotation, still 1 KB in a row.
+//
 // These products are bound by the power that the matrix cores draw, not by their rate: on random fp16 data (registers
 // and LDS alone) 16x16x32 reaches 1.81 PFLOP/s and 32x32x16 1.59, on zeros both 2.38. Hence the 16 x 16 form.
 #pragma once
@@ -36,7 +41,7 @@ struct Operand {
 // Where the hi plane's 8 values of row r, columns 8·o …, of a row group's step start (o: the octet of the 32 columns).
 template <int PLANES>
 __device__ __forceinline__ int unit_at(int r, int o) {
-    return ((r >> 4) * PLANES * 4 + o) * 128 + (r & 15) * 8;
+    return ((r >> 4) * PLANES * 4 + o) * 128 + ((r + 4 * o) & 15) * 8;
 }
 
 __device__ __forceinline__ void split_value(float v, _Float16& hi, _Float16& lo) {
@@ -68,13 +73,46 @@ __device__ __forceinline__ unsigned lds_byte(const void* p) {
     return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-// A workgroup of WAVES_M x WAVES_N waves, each BM x BN blocks of 16 x 16 outputs: C[m, n] += Σ_k A[m, k]·B[n, k].
+// One side's fragments as a wave reads them from a step in LDS. T: the operand's columns are the product's rows.
+template <int PLANES, bool T>
+struct Reader {
+    const _Float16* at[T ? 4 : 1];  // T: [16-column half][rows 4·p … 4·p + 3 of the lane's octet of rows]
+    __device__ __forceinline__ Reader(const _Float16* side, int lane) {
+        if constexpr (T) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int r = 8 * (lane >> 4) + 4 * (q & 1) + ((lane & 15) >> 2), c = lane & 3;
+                at[q] = side + unit_at<PLANES>(r, 2 * (q >> 1) + (c >> 1)) + 4 * (c & 1);
+            }
+        } else {
+            at[0] = side + unit_at<PLANES>(lane & 15, lane >> 4);
+        }
+    }
+    // Block i (16 of the product's rows), plane p, of the step `step` halves into the side's memory.
+    __device__ __forceinline__ f16x8 read(int step, int i, int p) const {
+        if constexpr (T) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            const int o = step + (i >> 1) * (2 * PLANES * FRAG) + p * FRAG;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(at[2 * (i & 1)] + o));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(at[2 * (i & 1) + 1] + o));
+            return __builtin_shufflevector(__builtin_bit_cast(f16x4, lo), __builtin_bit_cast(f16x4, hi), 0, 1, 2, 3, 4,
+                                           5, 6, 7);
+        } else {
+            return *reinterpret_cast<const f16x8*>(at[0] + step + (i * PLANES + p) * FRAG);
+        }
+    }
+};
+
+// A workgroup of WAVES_M x WAVES_N waves, each BM x BN blocks of 16 x 16 outputs: C[m, n] += Σ_k A[m, k]·B[n, k]. TA, TB:
+// that side is packed with the product's k as its rows.
 //
 // LDS holds two 32-deep steps. A step's barrier stands before its last row block's products: by then every wave has read
 // the step to the end and the next step's copies, started a step ago, have landed; behind it the copies of the step
 // after that start into the buffer just read, and the next step's first fragments are read while the last products run.
 // Between two barriers a wave has a whole step's products, and no read or copy is waited for where it is issued.
-template <int WAVES_M, int WAVES_N, int BM, int BN, int PA, int PB>
+template <int WAVES_M, int WAVES_N, int BM, int BN, int PA, int PB, bool TA = false, bool TB = false>
 struct Tile {
     static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
     static constexpr int M = WAVES_M * BM * 16, N = WAVES_N * BN * 16;
@@ -82,7 +120,8 @@ struct Tile {
     static constexpr int A_HALVES = MG * 2 * PA * FRAG, STEP = A_HALVES + NG * 2 * PB * FRAG;
     static constexpr int LDS_HALVES = 2 * STEP;
     static constexpr int PER_WAVE = (MG + NG) / WAVES;  // row groups a wave copies each step
-    static_assert((MG + NG) % WAVES == 0 && PER_WAVE <= 2 && (PA == PB || MG % WAVES == 0) && BM % 2 == 0, "tile shape");
+    static_assert((MG + NG) % WAVES == 0 && PER_WAVE <= 2 && BM % 2 == 0 && BN % 2 == 0 &&
+                      (MG % WAVES == 0 || (PA == PB && TA == TB)), "tile shape");
 
     typedef f32x4 Acc[BM][BN];
 
@@ -91,6 +130,7 @@ struct Tile {
 
     struct Copies {
         const _Float16* from[PER_WAVE];
+        size_t next[PER_WAVE];  // from a step to the next
         unsigned to[PER_WAVE];
         // Starts a step's copies into the buffer at byte `slot`, and moves on to the next step.
         __device__ __forceinline__ void start(unsigned slot) {
@@ -100,17 +140,19 @@ struct Tile {
         template <int C>
         __device__ __forceinline__ void copy(unsigned slot) {
             copy_to_lds<2 * planes(C)>(from[C], to[C] + slot);
-            from[C] += 2 * planes(C) * FRAG;
+            from[C] += next[C];
         }
     };
 
-    static __device__ __forceinline__ void read_a(const _Float16* step, int i, f16x8 (&a)[PA]) {
+    typedef Reader<PA, TA> ReadA;
+    typedef Reader<PB, TB> ReadB;
+    static __device__ __forceinline__ void read_a(const ReadA& as, int step, int i, f16x8 (&a)[PA]) {
 #pragma unroll
-        for (int p = 0; p < PA; ++p) a[p] = *reinterpret_cast<const f16x8*>(step + (i * PA + p) * FRAG);
+        for (int p = 0; p < PA; ++p) a[p] = as.read(step, i, p);
     }
-    static __device__ __forceinline__ void read_b(const _Float16* step, int j, f16x8 (&b)[PB]) {
+    static __device__ __forceinline__ void read_b(const ReadB& bs, int step, int j, f16x8 (&b)[PB]) {
 #pragma unroll
-        for (int p = 0; p < PB; ++p) b[p] = *reinterpret_cast<const f16x8*>(step + (j * PB + p) * FRAG);
+        for (int p = 0; p < PB; ++p) b[p] = bs.read(step, j, p);
     }
     // The pieces' products, smallest first: of a whole row block, piece by piece (no product waits for the one before),
     // and of one block.
@@ -145,40 +187,43 @@ struct Tile {
 #pragma unroll
         for (int c = 0; c < PER_WAVE; ++c) {
             const int i = __builtin_amdgcn_readfirstlane(wave + c * WAVES);
-            cp.from[c] =
-                i < MG ? a.data + ((size_t)min(mg0 + i, a.groups - 1) * a.steps + s0) * (2 * PA * FRAG) + lane * 8
-                       : b.data + ((size_t)min(ng0 + i - MG, b.groups - 1) * b.steps + s0) * (2 * PB * FRAG) + lane * 8;
-            cp.to[c] = lds0 + 2 * (i < MG ? i * (2 * PA * FRAG) : A_HALVES + (i - MG) * (2 * PB * FRAG));
+            const bool on_a = i < MG, turned = on_a ? TA : TB;
+            const Operand& o = on_a ? a : b;
+            const int at = on_a ? mg0 + i : ng0 + i - MG, size = 2 * (on_a ? PA : PB) * FRAG;
+            cp.from[c] = o.data + lane * 8 +
+                         (turned ? (size_t)s0 * o.steps + min(at, o.steps - 1)
+                                 : (size_t)min(at, o.groups - 1) * o.steps + s0) * size;
+            cp.next[c] = (turned ? (size_t)o.steps : (size_t)1) * size;
+            cp.to[c] = lds0 + 2 * (on_a ? i * size : A_HALVES + (i - MG) * size);
         }
-        const _Float16* as = lds + wm * BM * (PA * FRAG) + lane * 8;
-        const _Float16* bs = lds + A_HALVES + wn * BN * (PB * FRAG) + lane * 8;
+        const ReadA as(lds + wm * BM * (PA * FRAG), lane);
+        const ReadB bs(lds + A_HALVES + wn * BN * (PB * FRAG), lane);
         cp.start(0);
         wait_copies();
         if (s1 - s0 > 1) cp.start(2 * STEP);
         f16x8 fa[2][PA], fb[BN][PB];
-        read_a(as, 0, fa[0]);
+        read_a(as, 0, 0, fa[0]);
 #pragma unroll
-        for (int j = 0; j < BN; ++j) read_b(bs, j, fb[j]);
+        for (int j = 0; j < BN; ++j) read_b(bs, 0, j, fb[j]);
         // One step from buffer H (its fragments of B in fb, A's first in fa[0]); the last row block's products hand fb over
         // to the next step's, block by block. What is read ahead of the last step's end is of a buffer that no one needs.
         auto step = [&](auto buffer, bool more) {
-            constexpr int H = decltype(buffer)::value;
-            const _Float16 *at = as + H * STEP, *an = as + (H ^ 1) * STEP, *bn = bs + (H ^ 1) * STEP;
+            constexpr int H = decltype(buffer)::value, at = H * STEP, next = (H ^ 1) * STEP;
 #pragma unroll
             for (int i = 0; i + 1 < BM; ++i) {
-                read_a(at, i + 1, fa[(i + 1) & 1]);
+                read_a(as, at, i + 1, fa[(i + 1) & 1]);
                 __builtin_amdgcn_sched_barrier(0);
                 mma(fa[i & 1], fb, acc[i]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             wait_copies();
             if (more) cp.start(H * (2 * STEP));
-            read_a(an, 0, fa[0]);
+            read_a(as, next, 0, fa[0]);
 #pragma unroll
             for (int j = 0; j < BN; ++j) {
                 mma1(fa[1], fb[j], acc[BM - 1][j]);
                 __builtin_amdgcn_sched_barrier(0);
-                read_b(bn, j, fb[j]);
+                read_b(bs, next, j, fb[j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };

@@ -8,9 +8,9 @@
 // enough for the piece's two products. Rows without a label are dropped first (label_rows), so that a batch with labels
 // on 15 % of its tokens costs the products of those alone.
 //
-// Scales of the two-piece products (powers of two, so that scaling is exact): W by row (2^ea[v]), x by row (2^ex[t]);
-// G by 2^14. Where the product runs over v, G carries 2^(emin − ea[v]) beside it, which brings W's rows back to one
-// scale; where it runs over t, w_t·x_t has one scale for all.
+// Scales of the two-piece products (powers of two, so that scaling is exact): x by row, G by 2^14, w_t·x_t as a whole. W
+// by row in the forward; as a whole in the backward, where one packed W serves the logits (over its columns) and dx
+// (over its rows), as one packed G serves dx and dW.
 #include "elementwise.hpp"
 #include "packed.hpp"
 
@@ -25,9 +25,9 @@ constexpr int MAX_SPLITS = 16;       // ways of dx's sum over a piece of the voc
 constexpr size_t PIECE_BYTES = (size_t)3 << 30;  // of packed table and G that a piece of the vocabulary may take
 constexpr float LOG2E = 1.44269504088896341f;
 
-// Words of a call: [0] labelled rows, [1] targets outside the vocabulary, [2] bits of max|w_t·x_t|,
-// [3] the ways dx's sum is split; then a word a piece: 126 − min over its rows of ea (an atomicMax of a non-negative value).
-enum : int { WORD_COUNT = 0, WORD_BAD = 1, WORD_WX = 2, WORD_SPLITS = 3, WORD_PIECES = 4 };
+// Words of a call: labelled rows, targets outside the vocabulary, bits of max|w_t·x_t| and of max|W|, the ways that dx's
+// sum is split.
+enum : int { WORD_COUNT, WORD_BAD, WORD_WX, WORD_W, WORD_SPLITS, WORDS };
 
 // ------------------------------------------------------------------------------------------- labels
 
@@ -35,7 +35,7 @@ enum : int { WORD_COUNT = 0, WORD_BAD = 1, WORD_WX = 2, WORD_SPLITS = 3, WORD_PI
 // LAYA_NO_LABEL carries no label; any other outside [0, vocab) is counted and carries none either.
 __global__ __launch_bounds__(1024) void label_rows_kernel(const int* __restrict__ targets, int rows, int vocab,
                                                           int* __restrict__ row_of, int* __restrict__ place,
-                                                          unsigned* words, int n_words, int* bad_count, float* row_loss,
+                                                          unsigned* words, int* bad_count, float* row_loss,
                                                           float* lse) {
     __shared__ int wave_count[16], wave_bad[16];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(1024) void label_rows_kernel(const int* __restrict_
         }
         __syncthreads();
     }
-    for (int i = tid; i < n_words; i += 1024) words[i] = i == WORD_COUNT ? base : i == WORD_BAD ? bad : 0;
+    if (tid < WORDS) words[tid] = tid == WORD_COUNT ? base : tid == WORD_BAD ? bad : 0;
     if (tid == 0 && bad_count) *bad_count = bad;
 }
 
@@ -106,33 +106,29 @@ __device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v
 }
 
 struct PackRows {
-    const void* src;          // [.., K]
-    const int* row_of;        // source row of packed row j (null: j itself)
-    const unsigned* count;    // rows on the device (null: `rows`)
+    const void* src;         // [.., K]
+    const int* row_of;       // source row of packed row j (null: j itself)
+    const unsigned* count;   // rows on the device (null: `rows`)
     int rows, K;
-    int* exps;                // [rows padded to TILE]: the exponent of each row's scale
-    _Float16* out;            // rows as rows
-    _Float16* out_t;          // rows as k (null: not wanted)
-    int steps_t;
-    const float* bias;        // with `padded`: bias (or zeros) by row, −∞ behind the last
+    const unsigned* whole;   // bits of the operand's largest magnitude, its scale (null: each row has its own)
+    int* exps;               // [rows padded to TILE]: the exponent of each row's scale
+    _Float16* out;
+    const float* bias;       // with `padded`: bias (or zeros) by row, −∞ behind the last
     float* padded;
-    const float* weights;     // of the gathered source rows (null: 1), for `wx`
-    unsigned* wx;             // max |weight·x| as bits (null: not wanted)
-    unsigned* emin;           // 126 − min over the rows of exps (null: not wanted)
+    const float* weights;    // of the gathered source rows (null: 1), for `wx`
+    unsigned* wx;            // max |weight·x| as bits (null: not wanted)
 };
 
-// One workgroup packs 32 rows, each scaled so that its largest finite magnitude lies in [2^14, 2^15): one read for the
-// magnitudes, one (from the caches) for the pieces. Thread t holds 8 columns of row t / 8. T: fp32 or bf16 source.
+// One workgroup packs 32 rows, scaled so that the largest finite magnitude (a row's own, or the operand's) lies in
+// [2^14, 2^15). Row scales take one read for the magnitudes and one, from the caches, for the pieces. Thread t holds 8
+// columns of row t / 8. T: fp32 or bf16 source.
 template <typename T, int PLANES, bool VEC>
 __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
-    constexpr int CHUNK = 64, PITCH = CHUNK + 1;
-    __shared__ unsigned turn[32 * PITCH];
-    __shared__ int row_exp[32];
     const int b = blockIdx.x, tid = threadIdx.x, r = tid >> 3, o = tid & 7;
     const int rows = p.count ? (int)*p.count : p.rows;
     const int j = 32 * b + r;
-    if (32 * b >= rows) {  // behind the last block: what the tiles that reach over it read by row
-        if (o == 0 && p.padded && 32 * b < (p.rows + TILE - 1) / TILE * TILE) {
+    if (32 * b >= rows) {  // behind the last group: what the tiles that reach over it read by row
+        if (o == 0 && p.padded) {
             p.exps[j] = 0;
             p.padded[j] = -__builtin_inff();
         }
@@ -142,18 +138,21 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
     const int from = live ? (p.row_of ? p.row_of[j] : j) : 0;
     const T* row = static_cast<const T*>(p.src) + (size_t)from * p.K;
     unsigned am = 0;
-    if (live)
-        for (int c = o * 8; c < p.K; c += 64) {
-            float v[8];
-            load8<VEC>(row, c, p.K, v);
+    if (p.whole) {
+        am = *p.whole;
+    } else {
+        if (live)
+            for (int c = o * 8; c < p.K; c += 64) {
+                float v[8];
+                load8<VEC>(row, c, p.K, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) am = max(am, amax_bits(v[i]));
-        }
+                for (int i = 0; i < 8; ++i) am = max(am, amax_bits(v[i]));
+            }
 #pragma unroll
-    for (int s = 1; s < 8; s <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, s, 64));
+        for (int s = 1; s < 8; s <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, s, 64));
+    }
     const int e = pair_scale_exp(am);
     if (o == 0) {
-        row_exp[r] = live ? e : 126;
         if (p.exps) p.exps[j] = live ? e : 0;
         if (p.padded) p.padded[j] = live ? (p.bias ? p.bias[j] : 0.0f) : -__builtin_inff();
     }
@@ -164,23 +163,11 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
         for (int s = 8; s < 64; s <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, s, 64));
         if ((tid & 63) == 0 && m) atomicMax(p.wx, m);
     }
-    __syncthreads();
-    if (p.emin && tid < 32) {
-        int m = 126 - row_exp[tid];
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) m = max(m, __shfl_xor(m, s, 64));
-        if (tid == 0) atomicMax(p.emin, (unsigned)m);
-    }
     const float sc = exp2_int(e);
     const int steps = (p.K + 31) / 32;
-    for (int c0 = 0; c0 < p.K; c0 += CHUNK) {
-        float v[8];
-        const int c = c0 + o * 8, step = c >> 5;
-        if (live)
-            load8<VEC>(row, c, p.K, v);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int c = o * 8; c < steps * 32; c += 64) {
+        float v[8] = {};
+        if (live) load8<VEC>(row, c, p.K, v);
         f16x8 hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -189,33 +176,43 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
             hi[i] = h;
             lo[i] = l;
         }
-        if (step < steps) {
-            _Float16* at = p.out + ((size_t)b * steps + step) * (2 * PLANES * FRAG) + unit_at<PLANES>(r, o & 3);
-            *reinterpret_cast<f16x8*>(at) = hi;
-            if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = lo;
-        }
-        if (p.out_t) {
+        _Float16* at = p.out + ((size_t)b * steps + (c >> 5)) * (2 * PLANES * FRAG) + unit_at<PLANES>(r, o & 3);
+        *reinterpret_cast<f16x8*>(at) = hi;
+        if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = lo;
+    }
+}
+
+// max |x| over the finite values, as bits folded into *word.
+template <typename T>
+__global__ __launch_bounds__(256) void table_amax_kernel(const T* __restrict__ x, size_t n, unsigned* word) {
+    constexpr int V = 16 / sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(V)));
+    unsigned m = 0;
+    const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, all = (size_t)gridDim.x * 256;
+    const size_t nv = ((uintptr_t)x & 15u) == 0 ? n / V : 0;
+    const Vec* xv = reinterpret_cast<const Vec*>(x);
+    size_t i = at;
+    for (; i + 3 * all < nv; i += 4 * all) {
+        const Vec a = xv[i], b = xv[i + all], c = xv[i + 2 * all], d = xv[i + 3 * all];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                turn[r * PITCH + o * 8 + i] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)hi[i]) |
-                                              (unsigned)__builtin_bit_cast(unsigned short, (_Float16)lo[i]) << 16;
-            __syncthreads();
-            const int h = tid & 63, u = tid >> 6;  // column c0 + h, rows 8u … 8u + 7
-            f16x8 th, tl;
+        for (int k = 0; k < V; ++k)
+            m = max(m, max(max(amax_bits((float)a[k]), amax_bits((float)b[k])),
+                           max(amax_bits((float)c[k]), amax_bits((float)d[k]))));
+    }
+    for (; i < nv; i += all) {
+        const Vec a = xv[i];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned w = turn[(8 * u + i) * PITCH + h];
-                th[i] = __builtin_bit_cast(_Float16, (unsigned short)w);
-                tl[i] = __builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
-            }
-            const int hg = (c0 + h) >> 5;
-            if (hg < steps) {
-                _Float16* at = p.out_t + ((size_t)hg * p.steps_t + b) * (2 * PLANES * FRAG) + unit_at<PLANES>(h & 31, u);
-                *reinterpret_cast<f16x8*>(at) = th;
-                if constexpr (PLANES == 2) *reinterpret_cast<f16x8*>(at + FRAG) = tl;
-            }
-            __syncthreads();
-        }
+        for (int k = 0; k < V; ++k) m = max(m, amax_bits((float)a[k]));
+    }
+    for (i = nv * V + at; i < n; i += all) m = max(m, amax_bits((float)x[i]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+    __shared__ unsigned red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        m = max(max(red[0], red[1]), max(red[2], red[3]));
+        if (m) atomicMax(word, m);
     }
 }
 
@@ -402,15 +399,13 @@ __global__ __launch_bounds__(1024) void vocab_total_kernel(const float* __restri
 struct GradOut {
     const int *row_of, *targets;
     const float *lse, *weights;
-    const unsigned* emin;
-    _Float16* g;     // rows t, k = v: G·2^(G_SCALE + emin − ea[v])
-    _Float16* g_t;   // rows v, k = t: G·2^G_SCALE
-    int steps_v, steps_t, groups_v;
+    _Float16* g;     // rows t, columns v: G·2^G_SCALE
+    int steps_v, groups_t;
     float* db_part;  // [4 a token tile][padded piece] (null: no bias gradient)
     int db_pitch;
 };
 
-// A piece's G in both orders.
+// A piece's G, packed as it lies in the accumulators (a lane has four v of one t in a row).
 template <int PW, bool DB>
 __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g) {
     typedef Tile<2, 4, 8, 4, PW, 2> T;
@@ -419,9 +414,6 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
     const int count = (int)p.words[WORD_COUNT];
     const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
     p.x.groups = (count + 31) / 32;
-    const int emin = 126 - (int)*g.emin;
-    unsigned* turn = reinterpret_cast<unsigned*>(lds) + wave * TURN_DWORDS;
-    float* wl = reinterpret_cast<float*>(lds) + T::WAVES * TURN_DWORDS + wave * 64;
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
@@ -432,12 +424,14 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
         T::product(p.W, p.x, tv * T::MG, tt * T::NG, 0, p.W.steps, lds, acc, wave, lane);
         const int v = tv * TILE + wm * 128, t = tt * TILE + wn * 64;
         to_logits(p, acc, v, t, lane);
+        float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int at = t + 16 * j + (lane & 15);
             const bool live = at < count;
             const int r = live ? g.row_of[at] : 0;
             const float lse = live ? g.lse[r] : 0.0f;
+            if (DB) w[j] = live ? (g.weights ? g.weights[r] : 1.0f) : 0.0f;
             // The target's place among the lane's values: 16·i + e.
             const int y = (live ? g.targets[r] : -1) - (p.v0 + v + 4 * (lane >> 4));
 #pragma unroll
@@ -448,71 +442,48 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
                     x -= y == 16 * i + e ? 1.0f : 0.0f;
                     acc[i][j][e] = live ? x * (float)(1 << G_SCALE) : 0.0f;
                 }
-            if (DB && lane < 16) wl[16 * j + lane] = live ? (g.weights ? g.weights[r] : 1.0f) : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int vg = (v >> 5) + i;
-            if (vg >= g.groups_v) break;  // wave-uniform
-            float db[2] = {0.0f, 0.0f};
-            int fold[2][4];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int4 ew = *reinterpret_cast<const int4*>(p.ew + v + 32 * i + 16 * q + 4 * (lane >> 4));
-                fold[q][0] = emin - ew.x;
-                fold[q][1] = emin - ew.y;
-                fold[q][2] = emin - ew.z;
-                fold[q][3] = emin - ew.w;
-            }
+            if (vg >= g.steps_v) break;  // wave-uniform
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int tg = (t >> 5) + j;
-                if (tg >= g.steps_t) break;  // wave-uniform
+                if (tg >= g.groups_t) break;  // wave-uniform
                 f32x4 c[2][2];
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) c[q][k] = acc[2 * i + q][2 * j + k];
-                turn_write(c, turn, lane);
-                _Float16* at = g.g_t + ((size_t)vg * g.steps_t + tg) * (4 * FRAG) + lane * 8;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    f16x8 hi, lo;
-                    turn_read(turn, lane, q, hi, lo);
-                    *reinterpret_cast<f16x8*>(at + 2 * q * FRAG) = hi;
-                    *reinterpret_cast<f16x8*>(at + (2 * q + 1) * FRAG) = lo;
-                    if constexpr (DB) {
-                        const float* w = wl + 32 * j + (lane >> 4) * 8;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) db[q] = fmaf((float)hi[k] + (float)lo[k], w[k], db[q]);
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) c[q][k][e] = __builtin_amdgcn_ldexpf(c[q][k][e], fold[q][e]);
                 store_transposed(c, g.g + ((size_t)tg * g.steps_v + vg) * (4 * FRAG), lane);
             }
             if constexpr (DB) {
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    db[q] += __shfl_xor(db[q], 16, 64);
-                    db[q] += __shfl_xor(db[q], 32, 64);
-                    if (lane < 16) g.db_part[(size_t)(tt * 4 + wn) * g.db_pitch + vg * 32 + 16 * q + lane] = db[q];
+                    f32x4 db = {};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) db[e] = fmaf(acc[2 * i + q][j][e], w[j], db[e]);
+#pragma unroll
+                    for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) db[e] += __shfl_xor(db[e], o, 64);
+                    if ((lane & 15) == 0)
+                        *reinterpret_cast<f32x4*>(g.db_part + (size_t)(tt * 4 + wn) * g.db_pitch + vg * 32 + 16 * q +
+                                                  4 * (lane >> 4)) = db;
                 }
             }
         }
-        __syncthreads();
     }
 }
 
 struct GradProducts {
-    Operand g_t, wx;   // dW: rows v · rows h over t
-    Operand g, W_t;    // dx: rows t · rows h over v
+    Operand g;         // rows t, columns v
+    Operand wx;        // rows h, columns t: dW = gᵀ·wxᵀ over t
+    Operand W;         // rows v, columns h: dx = g·W over v
     unsigned* words;
-    const unsigned* emin;
     int vocab, hidden; // the piece's rows, the width
     float* dW;         // the piece's first row
     float scale;
@@ -549,8 +520,8 @@ __device__ __forceinline__ int dx_splits(int steps_v, int count, int cap_rows, i
 // Both products of a piece in one launch.
 template <int PW>
 __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) {
-    typedef Tile<2, 4, 8, 4, 2, 2> TE;
-    typedef Tile<2, 4, 8, 4, 2, PW> TX;
+    typedef Tile<2, 4, 8, 4, 2, 2, true, false> TE;
+    typedef Tile<2, 4, 8, 4, 2, PW, false, true> TX;
     __shared__ __attribute__((aligned(16))) _Float16 lds[TE::LDS_HALVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
     const int count = (int)p.words[WORD_COUNT];
@@ -558,7 +529,7 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
     const int tiles_t = (count + TILE - 1) / TILE, steps_v = p.g.steps;
     const int splits = p.cap_rows ? dx_splits(p.steps_first, count, p.cap_rows, p.units_first, p.tiles_h, gridDim.x) : 0;
     const int units_e = p.tiles_v * p.tiles_h, units = units_e + tiles_t * p.tiles_h * splits;
-    const int e_wx = -(G_SCALE + pair_scale_exp(p.words[WORD_WX])), e_w = -(G_SCALE + 126 - (int)*p.emin);
+    const int e_wx = -(G_SCALE + pair_scale_exp(p.words[WORD_WX])), e_w = -(G_SCALE + pair_scale_exp(p.words[WORD_W]));
     p.g.groups = (count + 31) / 32;
     if (blockIdx.x == 0 && threadIdx.x == 0) p.words[WORD_SPLITS] = splits;
     for (int n = 0;; ++n) {
@@ -568,7 +539,7 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
         typename TE::Acc acc;
         if (u < units_e) {
             const int tv = u / p.tiles_h, th = u - tv * p.tiles_h;
-            TE::product(p.g_t, p.wx, tv * TE::MG, th * TE::NG, 0, (count + 31) / 32, lds, acc, wave, lane);
+            TE::product(p.g, p.wx, tv * TE::MG, th * TE::NG, 0, (count + 31) / 32, lds, acc, wave, lane);
             const int v = tv * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -592,7 +563,7 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
             const int w = u - units_e, per = tiles_t * p.tiles_h, s = w / per, in = w - s * per;
             const int tt = in / p.tiles_h, th = in - tt * p.tiles_h;
             const int s0 = (int)((long)steps_v * s / splits), s1 = (int)((long)steps_v * (s + 1) / splits);
-            TX::product(p.g, p.W_t, tt * TX::MG, th * TX::NG, s0, s1, lds, acc, wave, lane);
+            TX::product(p.g, p.W, tt * TX::MG, th * TX::NG, s0, s1, lds, acc, wave, lane);
             const int t = tt * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
             float* out = p.dx_part + (size_t)s * tiles_t * TILE * p.hidden;
 #pragma unroll
@@ -659,25 +630,35 @@ void launch_pack(laya_ctx* ctx, const PackRows& p, int blocks) {
     check_launch("pack_rows_kernel");
 }
 
-void pack_table(laya_ctx* ctx, const VocabArgs& a, int v0, int vocab, int* exps, float* padded, _Float16* out,
-                _Float16* out_t, unsigned* emin) {
+// A piece of the table: its rows' scales are their own, or all the one that `whole` says.
+void pack_table(laya_ctx* ctx, const VocabArgs& a, int v0, int vocab, const unsigned* whole, int* exps, float* padded,
+                _Float16* out) {
     PackRows p{};
     p.src = a.W16 ? (const void*)(a.W16 + (size_t)v0 * a.hidden) : (const void*)(a.W + (size_t)v0 * a.hidden);
     p.rows = vocab;
     p.K = a.hidden;
+    p.whole = whole;
     p.exps = exps;
     p.out = out;
-    p.out_t = out_t;
-    p.steps_t = steps_of(vocab);
     p.bias = a.bias ? a.bias + v0 : nullptr;
     p.padded = padded;
-    p.emin = emin;
     const int blocks = (int)(pad_tile(vocab) / 32);
-    ProfileScope scope(ctx, "vocab_pack", 0.0, (a.W16 ? 2.0 : 4.0) * vocab * a.hidden * (out_t ? 3 : 2));
+    ProfileScope scope(ctx, "vocab_pack", 0.0, (a.W16 ? 2.0 : 4.0) * vocab * a.hidden * 2);
     if (a.W16)
         launch_pack<__bf16, 1>(ctx, p, blocks);
     else
         launch_pack<float, 2>(ctx, p, blocks);
+}
+
+void table_amax(laya_ctx* ctx, const VocabArgs& a, unsigned* word) {
+    const size_t n = (size_t)a.vocab * a.hidden;
+    ProfileScope scope(ctx, "vocab_amax", 0.0, (a.W16 ? 2.0 : 4.0) * n);
+    const dim3 grid(blocks_for(n, 16384, 2048));
+    if (a.W16)
+        LAYA_LAUNCH(table_amax_kernel<__bf16>, grid, dim3(256), 0, ctx->stream, a.W16, n, word);
+    else
+        LAYA_LAUNCH(table_amax_kernel<float>, grid, dim3(256), 0, ctx->stream, a.W, n, word);
+    check_launch("table_amax_kernel");
 }
 
 void pack_states(laya_ctx* ctx, const VocabArgs& a, const int* row_of, unsigned* words, int* exps, _Float16* out,
@@ -723,7 +704,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
     _Float16 *xp, *wp;
     float2* part;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
-        ws.take(words, WORD_PIECES);
+        ws.take(words, WORDS);
         ws.take(row_of, a.rows);
         ws.take(ex, pitch);
         ws.take(ew, piece);
@@ -733,12 +714,12 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
         ws.take(part, (size_t)tiles * pitch);
     });
     LAYA_LAUNCH(label_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, a.targets, a.rows, a.vocab, row_of,
-                (int*)nullptr, words, (int)WORD_PIECES, bad_count, row_loss, lse);
+                (int*)nullptr, words, bad_count, row_loss, lse);
     check_launch("label_rows_kernel");
     pack_states(ctx, a, row_of, words, ex, xp, false);
     for (int v0 = 0; v0 < a.vocab; v0 += piece) {
         const int n = std::min(piece, a.vocab - v0);
-        pack_table(ctx, a, v0, n, ew, padded, wp, nullptr, nullptr);
+        pack_table(ctx, a, v0, n, nullptr, ew, padded, wp);
         Logits p{{wp, steps_of(a.hidden), groups_of(n)}, {xp, steps_of(a.hidden), 0}, ew, ex, padded, words, v0, n,
                  (n + TILE - 1) / TILE};
         ProfileScope scope(ctx, "vocab_stats", 2.0 * a.rows * a.hidden * n, 0.0);
@@ -767,16 +748,15 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = steps_of(a.hidden);
     const int steps_t = steps_of(a.rows);
     const int piece =
-        piece_rows(a.vocab, (size_t)steps_h * 32 * 4 * planes + (size_t)steps_t * 32 * 8);
-    const int pieces = (a.vocab + piece - 1) / piece, n_words = WORD_PIECES + pieces;
+        piece_rows(a.vocab, (size_t)steps_h * 32 * 2 * planes + (size_t)steps_t * 32 * 4);
     const int cap_rows = std::max(pitch, std::min(MAX_SPLITS * pitch, 32768));
     const int tiles_t = pitch / TILE, tiles_h = (a.hidden + TILE - 1) / TILE;
     unsigned* words;
     int *row_of, *place, *ex, *ew;
     float *padded, *part, *db_part;
-    _Float16 *xp, *xt, *wp, *wt, *gp, *gt;
+    _Float16 *xp, *xt, *wp, *gp;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
-        ws.take(words, n_words);
+        ws.take(words, WORDS);
         ws.take(row_of, a.rows);
         ws.take(place, a.rows);
         ws.take(ex, pitch);
@@ -785,33 +765,30 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
         ws.take(xp, halves(a.rows, a.hidden, 2));
         ws.take(xt, halves(a.hidden, a.rows, 2));
         ws.take(wp, halves(piece, a.hidden, planes));
-        ws.take(wt, dx ? halves(a.hidden, piece, planes) : 0);
         ws.take(gp, halves(a.rows, piece, 2));
-        ws.take(gt, halves(piece, a.rows, 2));
         ws.take(part, dx ? (size_t)cap_rows * a.hidden : 0);
         ws.take(db_part, db ? (size_t)tiles_t * 4 * piece : 0);
     });
     if (!db) db_part = nullptr;
     LAYA_LAUNCH(label_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, a.targets, a.rows, a.vocab, row_of, place, words,
-                n_words, (int*)nullptr, (float*)nullptr, (float*)nullptr);
+                (int*)nullptr, (float*)nullptr, (float*)nullptr);
     check_launch("label_rows_kernel");
     pack_states(ctx, a, row_of, words, ex, xp, true);
     LAYA_LAUNCH(pack_weighted_kernel, dim3(groups_of(a.rows), (a.hidden + 63) / 64), dim3(256), 0, ctx->stream, a.x,
                 a.row_weights, row_of, words, a.hidden, xt, steps_t);
     check_launch("pack_weighted_kernel");
+    table_amax(ctx, a, words + WORD_W);
     int steps_v = 0, units_e = 0;
-    for (int v0 = 0, k = 0; v0 < a.vocab; v0 += piece, ++k) {
+    for (int v0 = 0; v0 < a.vocab; v0 += piece) {
         const int n = std::min(piece, a.vocab - v0), tiles_v = (n + TILE - 1) / TILE;
         // Every piece splits dx's sum as the first does, so that its partial sums meet the first's.
         if (v0 == 0) {
             steps_v = steps_of(n);
             units_e = dW ? tiles_v * tiles_h : 0;
         }
-        unsigned* emin = words + WORD_PIECES + k;
-        pack_table(ctx, a, v0, n, ew, padded, wp, dx ? wt : nullptr, emin);
+        pack_table(ctx, a, v0, n, words + WORD_W, ew, padded, wp);
         Logits p{{wp, steps_h, groups_of(n)}, {xp, steps_h, 0}, ew, ex, padded, words, v0, n, tiles_v};
-        GradOut g{row_of, a.targets, lse, a.row_weights, emin, gp, gt, steps_of(n), steps_t, groups_of(n), db_part,
-                  piece};
+        GradOut g{row_of, a.targets, lse, a.row_weights, gp, steps_of(n), steps_t, db_part, piece};
         {
             ProfileScope scope(ctx, "vocab_grad", 2.0 * a.rows * a.hidden * n, 0.0);
             const dim3 grid(workgroups(ctx)), block(512);
@@ -826,12 +803,10 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
             check_launch("vocab_grad_kernel");
         }
         GradProducts q{};
-        q.g_t = {gt, steps_t, groups_of(n)};
         q.wx = {xt, steps_t, groups_of(a.hidden)};
         q.g = {gp, steps_of(n), 0};
-        q.W_t = {wt, steps_of(n), groups_of(a.hidden)};
+        q.W = {wp, steps_h, groups_of(n)};
         q.words = words;
-        q.emin = emin;
         q.vocab = n;
         q.hidden = a.hidden;
         q.dW = dW ? dW + (size_t)v0 * a.hidden : nullptr;
