@@ -41,6 +41,7 @@ extern "C" {
 typedef struct laya_ctx laya_ctx;
 typedef struct laya_rotary laya_rotary;
 typedef struct laya_segments laya_segments;
+typedef struct laya_matrices laya_matrices;
 typedef struct laya_model laya_model;
 
 const char* laya_last_error(void);
@@ -275,6 +276,26 @@ int laya_grad_norm_status(laya_ctx* ctx);
 int laya_adamw(laya_ctx* ctx, float* params, float* grads, float* m, float* v, int n_groups, const size_t* begin,
                const size_t* end, const double* lr, double beta1, double beta2, double eps, double weight_decay,
                int step, const float* coef, int zero_grads);
+
+/* Newton-Schulz orthogonalisation of `count` matrices [rows, cols] one after another: each is brought to Frobenius norm 1
+ * and taken `steps` times through X <- aX + (bA + cA²)X, A = X·Xᵀ (over its short side), a = 3.4445, b = −4.7750,
+ * c = 2.0315, which pushes every singular value into about [0.7, 1.2] and keeps the singular vectors (five steps do for
+ * values above ≈ 1/400 of the norm; smaller ones grow by up to `a` a step). A zero matrix stays zero; a matrix with a
+ * non-finite value becomes non-finite. out may be x. Norms are summed in double; products are fp32-accurate two-piece
+ * fp16 products under every matmul precision. No counterpart in the reference, which has AdamW alone. */
+int laya_orthogonalize(laya_ctx* ctx, const float* x, int count, int rows, int cols, int steps, float* out);
+
+/* Matrices inside a flat arena, for laya_muon: matrix i is [rows[i], cols[i]] from element offset[i] (host arrays; no two
+ * overlap), its update scaled by multiplier[i] (NULL: 1). They may be of any shapes; equal ones share launches. */
+int laya_matrices_create(laya_ctx* ctx, const size_t* offset, const int* rows, const int* cols, const float* multiplier,
+                         int n, laya_matrices** out);
+int laya_matrices_destroy(laya_ctx* ctx, laya_matrices* matrices);
+/* A Muon step of those matrices (momentum orthogonalised by laya_orthogonalize's iteration), over flat arenas as
+ * laya_adamw's: m <- mu·m + coef·g; u = coef·g + mu·m with nesterov, m without; p <- p·(1 − lr·weight_decay) −
+ * lr·multiplier·orthogonalised(u). coef: the clip's coefficient (device, may be NULL = 1); zero_grads clears the matrices'
+ * gradients. Elements of the arenas outside the matrices are neither read nor written. No counterpart in the reference. */
+int laya_muon(laya_ctx* ctx, const laya_matrices* matrices, float* params, float* grads, float* momentum, double lr,
+              double mu, int nesterov, double weight_decay, int steps, const float* coef, int zero_grads);
 
 /* ---------------------------------------------- operand magnitude words (per-op binding state)
  *

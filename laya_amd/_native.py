@@ -129,6 +129,10 @@ SIGNATURES = {
     "laya_grad_norm": (c_int, [P, P, c_size, c_double, P, P]),
     "laya_grad_norm_status": (c_int, [P]),
     "laya_adamw": (c_int, [P, P, P, P, P, c_int, P, P, P, c_double, c_double, c_double, c_double, c_int, P, c_int]),
+    "laya_orthogonalize": (c_int, [P, P, c_int, c_int, c_int, c_int, P]),
+    "laya_matrices_create": (c_int, [P, P, P, P, P, c_int, PP]),
+    "laya_matrices_destroy": (c_int, [P, P]),
+    "laya_muon": (c_int, [P, P, P, P, P, c_double, c_double, c_int, c_double, c_int, P, c_int]),
     "laya_amax": (c_int, [P, P, c_size, P]),
     "laya_linear_fwd_w": (c_int, [P, P, c_int, c_int, P, c_int, P, P, P, P, P, P]),
     "laya_linear_bwd_w": (c_int, [P, P, P, c_int, c_int, c_int, P, P, P, P, P, P, P, P]),

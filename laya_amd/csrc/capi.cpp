@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <numeric>
 #include <vector>
 
 #include "elementwise.hpp"
@@ -971,6 +972,100 @@ int laya_adamw(laya_ctx* ctx, float* params, float* grads, float* m, float* v, i
         }
         adamw_arena(ctx, params, grads, m, v, n, g, (float)beta1, (float)beta2, (float)eps, (float)std::sqrt(c2), coef,
                     zero_grads);
+    });
+}
+
+static void check_matrix(const char* what, long rows, long cols) {
+    LAYA_REQUIRE(rows > 0 && cols > 0 && rows <= 1 << 20 && cols <= 1 << 20 && rows * cols < 1ll << 31,
+                 std::string(what) + ": a matrix of " + std::to_string(rows) + " x " + std::to_string(cols));
+}
+
+int laya_orthogonalize(laya_ctx* ctx, const float* x, int count, int rows, int cols, int steps, float* out) {
+    return guarded([&] {
+        require_ctx(ctx);
+        check_matrix("orthogonalize", rows, cols);
+        LAYA_REQUIRE(count >= 0 && (size_t)count * rows * cols < (size_t)1 << 40, "orthogonalize: bad count");
+        LAYA_REQUIRE(steps >= 1 && steps <= 100, "orthogonalize: 1 to 100 steps");
+        LAYA_REQUIRE(count == 0 || (x && out), "orthogonalize: null tensor");
+        DeviceScope device(ctx);
+        if (count) orthogonalize(ctx, x, count, rows, cols, steps, out);
+    });
+}
+
+int laya_matrices_create(laya_ctx* ctx, const size_t* offset, const int* rows, const int* cols, const float* multiplier,
+                         int n, laya_matrices** out) {
+    return guarded([&] {
+        require_ctx(ctx);
+        LAYA_REQUIRE(out && n >= 0 && (n == 0 || (offset && rows && cols)), "matrices: bad arguments");
+        for (int i = 0; i < n; ++i) {
+            check_matrix("matrices", rows[i], cols[i]);
+            LAYA_REQUIRE(!multiplier || std::isfinite(multiplier[i]), "matrices: a multiplier that is not finite");
+            LAYA_REQUIRE(offset[i] < (size_t)1 << 40, "matrices: an offset beyond 2^40");
+        }
+        std::vector<int> order(n);
+        std::iota(order.begin(), order.end(), 0);
+        std::sort(order.begin(), order.end(), [&](int a, int b) { return offset[a] < offset[b]; });
+        for (int i = 1; i < n; ++i) {
+            const int a = order[i - 1];
+            LAYA_REQUIRE(offset[a] + (size_t)rows[a] * cols[a] <= offset[order[i]], "matrices: two of them overlap");
+        }
+        std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
+            const long wa = (long)rows[a] * cols[a], wb = (long)rows[b] * cols[b];
+            return wa != wb ? wa > wb : rows[a] < rows[b];
+        });
+        DeviceScope device(ctx);
+        auto* m = new laya_matrices();
+        try {
+            for (int i : order) {
+                if (m->runs.empty() || m->runs.back().rows != rows[i] || m->runs.back().cols != cols[i])
+                    m->runs.push_back({rows[i], cols[i], 0, (int)m->offsets.size()});
+                m->runs.back().count++;
+                m->offsets.push_back(offset[i]);
+                m->multipliers.push_back(multiplier ? multiplier[i] : 1.0f);
+            }
+            m->d_offsets = static_cast<size_t*>(ctx->alloc(sizeof(size_t) * std::max(n, 1)));
+            m->d_multipliers = static_cast<float*>(ctx->alloc(sizeof(float) * std::max(n, 1)));
+            if (n) {  // the host vectors live as long as the handle, whose end waits for the stream
+                LAYA_HIP(hipMemcpyAsync(m->d_offsets, m->offsets.data(), sizeof(size_t) * n, hipMemcpyHostToDevice,
+                                        ctx->stream));
+                LAYA_HIP(hipMemcpyAsync(m->d_multipliers, m->multipliers.data(), sizeof(float) * n,
+                                        hipMemcpyHostToDevice, ctx->stream));
+            }
+        } catch (...) {
+            if (m->d_offsets) ctx->release(m->d_offsets);
+            if (m->d_multipliers) ctx->release(m->d_multipliers);
+            delete m;
+            throw;
+        }
+        *out = m;
+    });
+}
+
+int laya_matrices_destroy(laya_ctx* ctx, laya_matrices* matrices) {
+    return guarded([&] {
+        require_ctx(ctx);
+        if (!matrices) return;
+        DeviceScope device(ctx);
+        ctx->release(matrices->d_offsets);
+        ctx->release(matrices->d_multipliers);
+        delete matrices;
+    });
+}
+
+int laya_muon(laya_ctx* ctx, const laya_matrices* matrices, float* params, float* grads, float* momentum, double lr,
+              double mu, int nesterov, double weight_decay, int steps, const float* coef, int zero_grads) {
+    return guarded([&] {
+        require_ctx(ctx);
+        LAYA_REQUIRE(matrices, "muon: null matrices");
+        LAYA_REQUIRE(matrices->offsets.empty() || (params && grads && momentum), "muon: null arena");
+        LAYA_REQUIRE(std::isfinite(lr) && std::isfinite(weight_decay) && mu >= 0 && mu < 1,
+                     "muon: lr and weight_decay finite, mu in [0, 1)");
+        LAYA_REQUIRE(steps >= 1 && steps <= 100, "muon: 1 to 100 steps");
+        LAYA_REQUIRE(params != grads && params != momentum && (grads != momentum || !grads),
+                     "muon: params, grads and momentum are arenas of their own");
+        DeviceScope device(ctx);
+        muon_step(ctx, *matrices, params, grads, momentum, (float)lr, (float)mu, nesterov,
+                  (float)(1.0 - lr * weight_decay), steps, coef, zero_grads);
     });
 }
 

@@ -143,6 +143,18 @@ struct laya_rotary {
     float* sin_t = nullptr;
 };
 
+// Matrices of an arena (laya_matrices_create), equal shapes together, the largest first; the tables are in that order.
+struct laya_matrices {
+    struct Run {
+        int rows, cols, count, first;
+    };
+    std::vector<Run> runs;
+    std::vector<size_t> offsets;
+    std::vector<float> multipliers;
+    size_t* d_offsets = nullptr;
+    float* d_multipliers = nullptr;
+};
+
 namespace laya {
 
 // ------------------------------------------------------------------------------ device helpers
@@ -392,6 +404,11 @@ struct VocabArgs {
 };
 void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count);
 void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db);
+
+// Newton-Schulz orthogonalisation and the Muon step (muon.hip); p = decay·p − rate·multiplier·X.
+void orthogonalize(laya_ctx* ctx, const float* x, int count, int rows, int cols, int steps, float* out);
+void muon_step(laya_ctx* ctx, const laya_matrices& mats, float* params, float* grads, float* momentum, float rate,
+               float mu, int nesterov, float decay, int steps, const float* coef, int zero_grads);
 
 // Σ over rows of a [rows, n] matrix added into out[n], deterministic (bias gradients); amax (optional): max|x| folded
 // into that word group in the same pass. Returns whether it was: only the float4 path of more than 256 rows does.

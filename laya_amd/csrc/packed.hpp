@@ -66,9 +66,13 @@ __device__ __forceinline__ void copy_to_lds(const _Float16* from, unsigned to) {
             "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
             "global_load_lds_dwordx4 %1, off offset:1024" ::"s"(to), "v"(from) : "memory");
 }
-// Waits for the wave's copies (and its other memory accesses), then for the whole workgroup: what every wave copied is
-// in LDS, and every wave's reads before this point are done.
-__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Waits for all but the wave's last N copies (and its other memory accesses before them), then for the whole workgroup:
+// what every wave copied before its last N is in LDS, and every wave's reads before this point are done.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    static_assert(N < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ unsigned lds_byte(const void* p) {
     return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
@@ -108,20 +112,24 @@ struct Reader {
 // A workgroup of WAVES_M x WAVES_N waves, each BM x BN blocks of 16 x 16 outputs: C[m, n] += Σ_k A[m, k]·B[n, k]. TA, TB:
 // that side is packed with the product's k as its rows.
 //
-// LDS holds two 32-deep steps. A step's barrier stands before its last row block's products: by then every wave has read
-// the step to the end and the next step's copies, started a step ago, have landed; behind it the copies of the step
-// after that start into the buffer just read, and the next step's first fragments are read while the last products run.
-// Between two barriers a wave has a whole step's products, and no read or copy is waited for where it is issued.
-template <int WAVES_M, int WAVES_N, int BM, int BN, int PA, int PB, bool TA = false, bool TB = false>
+// LDS holds a ring of 32-deep steps. A step's barrier stands before its last row block's products: by then every wave has
+// read the step to the end and the next step's copies, started RING − 1 steps ago, have landed; behind it the copies of
+// the step RING ahead start into the buffer just read, and the next step's first fragments are read while the last
+// products run. Between two barriers a wave has a whole step's products, and no read or copy is waited for where it is
+// issued. Two steps fill LDS with 256 x 256 tiles (and a step is long enough for a copy); small tiles, whose steps are
+// shorter than a copy takes, look further ahead.
+template <int WAVES_M, int WAVES_N, int BM, int BN, int PA, int PB, bool TA = false, bool TB = false, int RING = 2>
 struct Tile {
     static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
     static constexpr int M = WAVES_M * BM * 16, N = WAVES_N * BN * 16;
     static constexpr int MG = M / 32, NG = N / 32;  // row groups of A and B in a tile
     static constexpr int A_HALVES = MG * 2 * PA * FRAG, STEP = A_HALVES + NG * 2 * PB * FRAG;
-    static constexpr int LDS_HALVES = 2 * STEP;
+    static constexpr int LDS_HALVES = RING * STEP;
     static constexpr int PER_WAVE = (MG + NG) / WAVES;  // row groups a wave copies each step
     static_assert((MG + NG) % WAVES == 0 && PER_WAVE <= 2 && BM % 2 == 0 && BN % 2 == 0 &&
-                      (MG % WAVES == 0 || (PA == PB && TA == TB)), "tile shape");
+                      (MG % WAVES == 0 || PA == PB), "tile shape");
+
+    static constexpr int COPIES = MG % WAVES == 0 ? MG / WAVES * 2 * PA + NG / WAVES * 2 * PB : PER_WAVE * 2 * PA;
 
     typedef f32x4 Acc[BM][BN];
 
@@ -198,17 +206,22 @@ struct Tile {
         }
         const ReadA as(lds + wm * BM * (PA * FRAG), lane);
         const ReadB bs(lds + A_HALVES + wn * BN * (PB * FRAG), lane);
-        cp.start(0);
-        wait_copies();
-        if (s1 - s0 > 1) cp.start(2 * STEP);
+        const int len = s1 - s0;
+#pragma unroll
+        for (int q = 0; q < RING; ++q)
+            if (q < len) cp.start(q * (2 * STEP));
+        if (len >= RING)
+            wait_copies<(RING - 1) * COPIES>();
+        else
+            wait_copies<0>();
         f16x8 fa[2][PA], fb[BN][PB];
         read_a(as, 0, 0, fa[0]);
 #pragma unroll
         for (int j = 0; j < BN; ++j) read_b(bs, 0, j, fb[j]);
-        // One step from buffer H (its fragments of B in fb, A's first in fa[0]); the last row block's products hand fb over
-        // to the next step's, block by block. What is read ahead of the last step's end is of a buffer that no one needs.
-        auto step = [&](auto buffer, bool more) {
-            constexpr int H = decltype(buffer)::value, at = H * STEP, next = (H ^ 1) * STEP;
+        // One step from the buffer at `at` (its fragments of B in fb, A's first in fa[0]); the last row block's products hand
+        // fb over to the next step's, block by block. `ahead`: the steps behind it. What is read ahead of the last step's
+        // end is of a buffer that no one needs.
+        auto step = [&](int at, int next, int ahead) {
 #pragma unroll
             for (int i = 0; i + 1 < BM; ++i) {
                 read_a(as, at, i + 1, fa[(i + 1) & 1]);
@@ -216,8 +229,11 @@ struct Tile {
                 mma(fa[i & 1], fb, acc[i]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            wait_copies();
-            if (more) cp.start(H * (2 * STEP));
+            if (RING == 2 || ahead < RING)
+                wait_copies<0>();
+            else
+                wait_copies<(RING - 2) * COPIES>();
+            if (ahead >= RING) cp.start(2 * at);
             read_a(as, next, 0, fa[0]);
 #pragma unroll
             for (int j = 0; j < BN; ++j) {
@@ -227,14 +243,20 @@ struct Tile {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        const std::integral_constant<int, 0> first;
-        const std::integral_constant<int, 1> second;
-        int s = s0;
-        for (; s + 1 < s1; s += 2) {
-            step(first, s + 2 < s1);
-            step(second, s + 3 < s1);
+        int left = len;
+        if constexpr (RING == 2) {
+            for (; left > 1; left -= 2) {
+                step(0, STEP, left - 1);
+                step(STEP, 0, left - 2);
+            }
+            if (left > 0) step(0, STEP, 0);
+        } else {
+            for (int at = 0; left > 0; --left) {
+                const int next = at + STEP == RING * STEP ? 0 : at + STEP;
+                step(at, next, left - 1);
+                at = next;
+            }
         }
-        if (s < s1) step(first, false);
         __syncthreads();
     }
 };

@@ -434,6 +434,63 @@ def rlcd_objective(ctx: Context, logits: DeviceArray, targets: DeviceArray, opti
     return tuple(float(v) for v in out), grad
 
 
+# ------------------------------------------------------------------- orthogonalised momentum (Muon)
+
+def orthogonalize(ctx: Context, x: DeviceArray, count: int, rows: int, cols: int, out: DeviceArray,
+                  steps: int = 5) -> None:
+    """Newton-Schulz orthogonalisation of `count` matrices [rows, cols] one after another; out may be x
+    (laya_orthogonalize)."""
+    if count < 0 or min(x.size, out.size) < count * rows * cols:
+        raise ValueError(f"orthogonalize: x {x.shape} and out {out.shape} for {count} matrices of {rows} x {cols}")
+    check(lib().laya_orthogonalize(_h(ctx), x.ptr, count, rows, cols, steps, out.ptr))
+
+
+class MuonMatrices:
+    """The matrices of flat arenas that a Muon step moves: matrix i is [rows[i], cols[i]] from element offsets[i], its
+    update scaled by multipliers[i] (1 when None). Uploaded once, as a laya_matrices handle."""
+
+    def __init__(self, ctx: Context, offsets: Sequence[int], rows: Sequence[int], cols: Sequence[int],
+                 multipliers: Optional[Sequence[float]] = None):
+        import ctypes
+        n = len(offsets)
+        if len(rows) != n or len(cols) != n or (multipliers is not None and len(multipliers) != n):
+            raise ValueError(f"muon: {n} offsets, {len(rows)} rows and {len(cols)} columns")
+        if n and min(offsets) < 0:
+            raise ValueError("muon: a negative offset")
+        self.ctx = ctx
+        self.count = n
+        self.end = max((int(o) + int(r) * int(c) for o, r, c in zip(offsets, rows, cols)), default=0)
+        o, r, c = np.array(offsets, np.uint64), np.array(rows, np.int32), np.array(cols, np.int32)
+        k = None if multipliers is None else np.array(multipliers, np.float32)
+        h = ctypes.c_void_p()
+        check(lib().laya_matrices_create(_h(ctx), ptr(o), ptr(r), ptr(c), ptr(k), n, ctypes.byref(h)))
+        self.handle = h.value
+        ctx.register(self)
+
+    def close(self) -> None:
+        if getattr(self, "handle", None) and getattr(self.ctx, "handle", None):
+            lib().laya_matrices_destroy(self.ctx.handle, self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def muon(matrices: MuonMatrices, params: DeviceArray, grads: DeviceArray, momentum: DeviceArray, learning_rate: float,
+         mu: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+         coef: Optional[DeviceArray] = None, zero_grads: bool = False) -> None:
+    """A Muon step of the arenas' matrices: momentum, its Newton-Schulz orthogonalisation, decoupled decay and the update,
+    in place (laya_muon). The rest of the arenas is left alone."""
+    if min(params.size, grads.size, momentum.size) < matrices.end:
+        raise ValueError(f"muon: arenas of {params.size}, {grads.size} and {momentum.size} elements for matrices up to "
+                         f"{matrices.end}")
+    check(lib().laya_muon(_h(matrices.ctx), matrices.handle, params.ptr, grads.ptr, momentum.ptr, learning_rate, mu,
+                          int(nesterov), weight_decay, steps, ptr(coef), int(zero_grads)))
+
+
 def layer_norm_eps_default() -> float:
     return 1e-5
 
