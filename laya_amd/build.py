@@ -18,7 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "liblaya_hip.so")
 SOURCES = ["gemm.hip", "gemm_short.hip", "norm.hip", "attention.hip", "elementwise.hip", "optim.hip", "objective.hip",
-           "readout.hip", "vocab.hip", "muon.hip", "capi.cpp", "model.cpp"]
+           "readout.hip", "vocab.hip", "vocab_few.hip", "muon.hip",
+           "capi.cpp", "model.cpp"]
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
          "-packed-fp32-ops", "-Wall", "-Wno-unused-function", "-Wno-unused-result"]

@@ -13,6 +13,7 @@
 // (over its rows), as one packed G serves dx and dW.
 #include "elementwise.hpp"
 #include "packed.hpp"
+#include "vocab.hpp"
 
 namespace laya {
 namespace {
@@ -23,11 +24,6 @@ constexpr int TILE = 256;            // logits, G and both gradient products run
 constexpr int G_SCALE = 14;          // |G| ≤ 1
 constexpr int MAX_SPLITS = 16;       // ways of dx's sum over a piece of the vocabulary
 constexpr size_t PIECE_BYTES = (size_t)3 << 30;  // of packed table and G that a piece of the vocabulary may take
-constexpr float LOG2E = 1.44269504088896341f;
-
-// Words of a call: labelled rows, targets outside the vocabulary, bits of max|w_t·x_t| and of max|W|, the ways that dx's
-// sum is split.
-enum : int { WORD_COUNT, WORD_BAD, WORD_WX, WORD_W, WORD_SPLITS, WORDS };
 
 // ------------------------------------------------------------------------------------------- labels
 
@@ -74,36 +70,6 @@ __global__ __launch_bounds__(1024) void label_rows_kernel(const int* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------ packing
-
-// Eight consecutive values of a row from column c, zeros behind K. VEC: rows start on 16 bytes and K is a multiple of 8.
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* row, int c, int K, float (&v)[8]) {
-    if constexpr (VEC) {
-        const f32x4 zero = {};
-        const f32x4 a = c < K ? *reinterpret_cast<const f32x4*>(row + c) : zero;
-        const f32x4 b = c < K ? *reinterpret_cast<const f32x4*>(row + c + 4) : zero;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? row[c + i] : 0.0f;
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v)[8]) {
-    if constexpr (VEC) {
-        const bf16x8 zero = {};
-        const bf16x8 a = c < K ? *reinterpret_cast<const bf16x8*>(row + c) : zero;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)row[c + i] : 0.0f;
-    }
-}
 
 struct PackRows {
     const void* src;         // [.., K]
@@ -346,54 +312,57 @@ __global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* _
     }
 }
 
-// One wave a labelled row: the tiles' statistics merged, and the target's logit from W's row itself.
+// One wave a labelled row: the tiles' statistics merged, and the target's logit from W's row itself. The last workgroup to
+// end sums the rows' weighted losses, in their order.
 template <typename TW>
 __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restrict__ part, int pitch, int tiles,
-                                                          const unsigned* words, const int* __restrict__ row_of,
+                                                          unsigned* words, const int* __restrict__ row_of,
                                                           const int* __restrict__ targets, const float* __restrict__ x,
                                                           const TW* __restrict__ W, const float* __restrict__ bias,
-                                                          int hidden, float* __restrict__ row_loss,
-                                                          float* __restrict__ lse) {
-    const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (j >= (int)words[WORD_COUNT]) return;
-    const int r = row_of[j], y = targets[r];
-    float m = -__builtin_inff();
-    for (int k = lane; k < tiles; k += 64) m = fmaxf(m, part[(size_t)k * pitch + j].x);
+                                                          int hidden, float* row_loss, float* __restrict__ lse,
+                                                          const float* __restrict__ weights, float scale, float* loss) {
+    const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, count = (int)words[WORD_COUNT];
+    if (j < count) {
+        const int r = row_of[j], y = targets[r];
+        float m = -__builtin_inff();
+        for (int k = lane; k < tiles; k += 64) m = fmaxf(m, part[(size_t)k * pitch + j].x);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    double s = 0.0, z = 0.0;
-    for (int k = lane; k < tiles; k += 64) {
-        const float2 a = part[(size_t)k * pitch + j];
-        if (a.y != 0.0f) s += (double)a.y * exp((double)a.x - (double)m);
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        double s = 0.0, z = 0.0;
+        for (int k = lane; k < tiles; k += 64) {
+            const float2 a = part[(size_t)k * pitch + j];
+            if (a.y != 0.0f) s += (double)a.y * exp((double)a.x - (double)m);
+        }
+        for (int k = lane; k < hidden; k += 64)
+            z += (double)x[(size_t)r * hidden + k] * (double)(float)W[(size_t)y * hidden + k];
+        s = wave_sum_d(s);
+        z = wave_sum_d(z);
+        if (lane == 0) {
+            const double l = (double)m + log(s);
+            lse[r] = (float)l;
+            __hip_atomic_store(row_loss + r, (float)(l - (z + (bias ? (double)bias[y] : 0.0))), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
-    for (int k = lane; k < hidden; k += 64) z += (double)x[(size_t)r * hidden + k] * (double)(float)W[(size_t)y * hidden + k];
-    s = wave_sum_d(s);
-    z = wave_sum_d(z);
-    if (lane == 0) {
-        const double l = (double)m + log(s);
-        lse[r] = (float)l;
-        row_loss[r] = (float)(l - (z + (bias ? (double)bias[y] : 0.0)));
-    }
-}
-
-// Σ w_r·loss_r·scale over the labelled rows, in a fixed order.
-__global__ __launch_bounds__(1024) void vocab_total_kernel(const float* __restrict__ row_loss, const unsigned* words,
-                                                           const int* __restrict__ row_of,
-                                                           const float* __restrict__ weights, float scale, float* loss) {
-    __shared__ double red[16];
-    const int count = (int)words[WORD_COUNT];
-    double s = 0.0;
-    for (int j = threadIdx.x; j < count; j += 1024) {
-        const int r = row_of[j];
-        s += (double)row_loss[r] * (weights ? (double)weights[r] : 1.0);
-    }
-    s = wave_sum_d(s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if (!loss) return;
+    __shared__ unsigned last;
+    __shared__ double red[4];
+    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) s += red[w];
-        *loss = (float)(s * (double)scale);
+    if (threadIdx.x == 0) last = atomicAdd(words + WORD_ENDED, 1u) + 1 == gridDim.x;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double s = 0.0;
+    for (int k = threadIdx.x; k < count; k += 256) {
+        const int r = row_of[k];
+        s += (double)__hip_atomic_load(row_loss + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) *
+             (weights ? (double)weights[r] : 1.0);
     }
+    s = wave_sum_d(s);
+    if (lane == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) *loss = (float)(((red[0] + red[1]) + (red[2] + red[3])) * (double)scale);
 }
 
 struct GradOut {
@@ -689,12 +658,25 @@ int workgroups(const laya_ctx* ctx) { return std::max(8, ctx->cu_count / 8 * 8);
 
 }  // namespace
 
+void vocab_merge(laya_ctx* ctx, const VocabArgs& a, const float2* part, int pitch, int tiles, unsigned* words,
+                 const int* row_of, float* row_loss, float* lse, float* loss) {
+    const dim3 grid((a.rows + 3) / 4);
+    if (a.W16)
+        LAYA_LAUNCH(vocab_merge_kernel<__bf16>, grid, dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
+                    a.targets, a.x, a.W16, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale, loss);
+    else
+        LAYA_LAUNCH(vocab_merge_kernel<float>, grid, dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
+                    a.targets, a.x, a.W, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale, loss);
+    check_launch("vocab_merge_kernel");
+}
+
 void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count) {
     if (a.rows == 0) {
         if (loss) fill(ctx, loss, 0.0f, 1);
         if (bad_count) fill(ctx, reinterpret_cast<float*>(bad_count), 0.0f, 1);
         return;
     }
+    if (a.rows <= VOCAB_FEW) return vocab_few_fwd(ctx, a, row_loss, lse, loss, bad_count);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
     const int piece = piece_rows(a.vocab, (size_t)steps_of(a.hidden) * 32 * 2 * planes);
     const int tiles = (a.vocab + TILE - 1) / TILE;
@@ -729,22 +711,12 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
             LAYA_LAUNCH(vocab_stats_kernel<2>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, p, part, pitch);
         check_launch("vocab_stats_kernel");
     }
-    if (a.W16)
-        LAYA_LAUNCH(vocab_merge_kernel<__bf16>, dim3((a.rows + 3) / 4), dim3(256), 0, ctx->stream, part, pitch, tiles,
-                    words, row_of, a.targets, a.x, a.W16, a.bias, a.hidden, row_loss, lse);
-    else
-        LAYA_LAUNCH(vocab_merge_kernel<float>, dim3((a.rows + 3) / 4), dim3(256), 0, ctx->stream, part, pitch, tiles,
-                    words, row_of, a.targets, a.x, a.W, a.bias, a.hidden, row_loss, lse);
-    check_launch("vocab_merge_kernel");
-    if (loss) {
-        LAYA_LAUNCH(vocab_total_kernel, dim3(1), dim3(1024), 0, ctx->stream, row_loss, words, row_of, a.row_weights,
-                    a.scale, loss);
-        check_launch("vocab_total_kernel");
-    }
+    vocab_merge(ctx, a, part, pitch, tiles, words, row_of, row_loss, lse, loss);
 }
 
 void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {
     if (a.rows == 0) return;
+    if (a.rows <= VOCAB_FEW) return vocab_few_bwd(ctx, a, lse, dx, dW, db);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = steps_of(a.hidden);
     const int steps_t = steps_of(a.rows);
     const int piece =
