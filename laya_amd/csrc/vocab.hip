@@ -324,21 +324,31 @@ __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restri
     const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, count = (int)words[WORD_COUNT];
     if (j < count) {
         const int r = row_of[j], y = targets[r];
-        float m = -__builtin_inff();
-        for (int k = lane; k < tiles; k += 64) m = fmaxf(m, part[(size_t)k * pitch + j].x);
+        double z = 0.0;
+        // Each lane's tiles, four at a time: the maximum and the sum so far.
+        float m = -__builtin_inff(), s = 0.0f;
+        for (int k = lane; k < tiles; k += 256) {
+            float2 a[4];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        double s = 0.0, z = 0.0;
-        for (int k = lane; k < tiles; k += 64) {
-            const float2 a = part[(size_t)k * pitch + j];
-            if (a.y != 0.0f) s += (double)a.y * exp((double)a.x - (double)m);
+            for (int q = 0; q < 4; ++q)
+                a[q] = k + 64 * q < tiles ? part[(size_t)(k + 64 * q) * pitch + j] : make_float2(-__builtin_inff(), 0.0f);
+            const float top = fmaxf(fmaxf(m, fmaxf(a[0].x, a[1].x)), fmaxf(a[2].x, a[3].x));
+            const float at = top == -__builtin_inff() ? 0.0f : top;
+            s *= __builtin_amdgcn_exp2f((m - at) * LOG2E);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s = fmaf(a[q].y, __builtin_amdgcn_exp2f((a[q].x - at) * LOG2E), s);
+            m = top;
         }
         for (int k = lane; k < hidden; k += 64)
             z += (double)x[(size_t)r * hidden + k] * (double)(float)W[(size_t)y * hidden + k];
-        s = wave_sum_d(s);
+        float top = m;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        const float at = top == -__builtin_inff() ? 0.0f : top;
+        const double sum = wave_sum_d((double)(s * __builtin_amdgcn_exp2f((m - at) * LOG2E)));
         z = wave_sum_d(z);
         if (lane == 0) {
-            const double l = (double)m + log(s);
+            const double l = (double)top + log(sum);
             lse[r] = (float)l;
             __hip_atomic_store(row_loss + r, (float)(l - (z + (bias ? (double)bias[y] : 0.0))), __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);

@@ -18,8 +18,6 @@ namespace {
 using packed::FRAG;
 using packed::lds_byte;
 
-constexpr int FEW_V = 128;  // rows of W a workgroup of few_logits takes
-
 __device__ __forceinline__ void split8(const float (&v)[8], bf16x8 (&p)[3]) {
     bf16x4 a[3], b[3];
     split3_4(f32x4{v[0], v[1], v[2], v[3]}, a[0], a[1], a[2]);
@@ -139,31 +137,49 @@ __global__ __launch_bounds__(256) void few_prepare_kernel(Prepare p) {
 
 // ------------------------------------------------------------------------------------------- shared
 
-// Fragments that all waves of a workgroup read, copied to an LDS ring a step at a time: NB·3 KB in a row a step, each
-// wave starting PER copies of 1 KB (the last ones may repeat one: the same bytes to the same place).
-template <int NB, int WAVES, int RING>
+// Fragments that all waves of a workgroup read, copied to an LDS ring a step at a time: KB KB in a row a step, each of at
+// least WAVES waves starting PER copies of 1 KB (some may repeat the last: the same bytes to the same place).
+template <int KB, int WAVES, int RING>
 struct Stream {
-    static constexpr int KB = 3 * NB, PER = (KB + WAVES - 1) / WAVES, STEP = KB * FRAG;
+    static constexpr int PER = (KB + WAVES - 1) / WAVES, STEP = KB * FRAG;
     const __bf16* from;
     unsigned lds0;
     int chunk[PER], last;
     __device__ __forceinline__ Stream(const __bf16* data, const __bf16* lds, int wave, int lane, int steps)
         : from(data + lane * 8), lds0(lds_byte(lds)), last(steps - 1) {
 #pragma unroll
-        for (int k = 0; k < PER; ++k) chunk[k] = __builtin_amdgcn_readfirstlane(min(wave + k * WAVES, KB - 1));
+        for (int k = 0; k < PER; ++k) chunk[k] = __builtin_amdgcn_readfirstlane(min(wave + k * (int)(blockDim.x >> 6), KB - 1));
     }
     // Step s into its slot; past the end the last step again, so that each step has as many copies under way.
     __device__ __forceinline__ void start(int s) const {
         const size_t at = (size_t)min(s, last) * STEP;
         const unsigned slot = lds0 + (unsigned)(s % RING) * (2 * STEP);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const unsigned to = slot + chunk[k] * (2 * FRAG);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to),
-                         "v"(from + at + chunk[k] * FRAG) : "memory");
-        }
+        for (int k = 0; k < PER; ++k) copy(at, slot, k);
+    }
+    // The same without the repeated copies, for who waits for all.
+    __device__ __forceinline__ void start_once(int s, int wave) const {
+        const size_t at = (size_t)s * STEP;
+        const unsigned slot = lds0 + (unsigned)(s % RING) * (2 * STEP);
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (__builtin_amdgcn_readfirstlane(wave) + k * (int)(blockDim.x >> 6) < KB) copy(at, slot, k);
+    }
+    __device__ __forceinline__ void copy(size_t at, unsigned slot, int k) const {
+        const unsigned to = slot + chunk[k] * (2 * FRAG);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to),
+                     "v"(from + at + chunk[k] * FRAG) : "memory");
     }
 };
+
+// Few-row products run in steps of 32 k with RING slots: step s starts the copies and the wave's own loads (LOADS of them,
+// each an instruction) of step s + RING − 1. What a wave has started behind the copies of step s when it comes to it:
+// the loads of steps s … s + RING − 2 and the copies of s + 1 … s + RING − 2. Waiting until no more than these are under
+// way means that the copies have landed; memory accesses end in order.
+template <int RING, int PER, int LOADS>
+__device__ __forceinline__ void wait_step() {
+    packed::wait_copies<(RING - 1) * LOADS + (RING - 2) * PER>();
+}
 
 // ------------------------------------------------------------------------------------------- logits
 
@@ -172,9 +188,9 @@ struct FewLogits {
     const float* bias;
     const __bf16* x_rows;
     const unsigned* words;
-    int hidden, vocab, steps;
+    int hidden, vocab, steps, blocks_v;  // blocks_v: blocks of 16 rows of W, an even number
     // Statistics:
-    float2* part;            // [tile of FEW_V][pitch]
+    float2* part;            // [workgroup][pitch]
     int pitch;
     // G:
     const int *row_of, *targets;
@@ -185,31 +201,65 @@ struct FewLogits {
     float scale;
 };
 
-constexpr int AHEAD = 4;  // steps of W that a wave has under way
+constexpr int RING = 4;
 
-template <int NB, typename TW, bool VEC, bool GRAD>
-__global__ __launch_bounds__(512, 2) void few_logits_kernel(FewLogits p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 3, RING = 4;
-    typedef Stream<NB, 8, RING> S;
-    __shared__ __attribute__((aligned(16))) __bf16 lds[RING * S::STEP < 16384 ? 16384 : RING * S::STEP];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, steps = p.steps;
-    const int v0 = blockIdx.x * FEW_V + wave * 16;
+// load8 as two loads (fp32) or one (bf16) whatever the column (aligned rows of a multiple of 8); the caller clears what lies
+// behind K.
+__device__ __forceinline__ void load8_always(const float* row, int c, int K, float (&v)[8]) {
+    const int at = c < K ? c : 0;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(row + at), b = *reinterpret_cast<const f32x4*>(row + at + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+    }
+}
+__device__ __forceinline__ void load8_always(const __bf16* row, int c, int K, float (&v)[8]) {
+    const bf16x8 a = *reinterpret_cast<const bf16x8*>(row + (c < K ? c : 0));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+}
+
+// A workgroup is as many waves, WAVES at least, as spread the table's blocks of 16 rows evenly over the CUs.
+template <int NB, typename TW, bool VEC, bool GRAD, int WAVES>
+__global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 3, LOADS = sizeof(TW) == 2 ? 1 : 2;
+    typedef Stream<3 * NB, WAVES, RING> S;
+    constexpr int PITCH = 36, ROOM = GRAD ? 16 * 16 * PITCH * 2 : 16 * 16 * NB * 4;  // what the end needs
+    __shared__ __attribute__((aligned(16))) __bf16 lds[RING * S::STEP < ROOM ? ROOM : RING * S::STEP];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, waves = blockDim.x >> 6, steps = p.steps;
+    const int v0 = (blockIdx.x * waves + wave) * 16;
     const TW* row = static_cast<const TW*>(p.W) + (size_t)min(v0 + (lane & 15), p.vocab - 1) * p.hidden;
     const S x(p.x_rows, lds, wave, lane, steps);
-    float w[AHEAD][8];
+    auto load = [&](int s, float (&w)[8]) {
+        const int c = 32 * s + 8 * (lane >> 4);
+        if constexpr (VEC)
+            load8_always(row, c, p.hidden, w);
+        else
+            load8<false>(row, c, p.hidden, w);
+    };
+    float w[RING][8];
     f32x4 acc[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[j] = f32x4{};
 #pragma unroll
-    for (int k = 0; k < RING - 1; ++k) x.start(k);
-#pragma unroll
-    for (int k = 0; k < AHEAD - 1; ++k) load8<VEC>(row, 32 * k + 8 * (lane >> 4), p.hidden, w[k]);
+    for (int k = 0; k < RING - 1; ++k) {
+        x.start(k);
+        load(k, w[k]);
+    }
     auto step = [&](int s, auto slot) {
         constexpr int K = decltype(slot)::value;
         // Step s's copies have landed for every wave, and step s − 1 is read by all: its slot is free.
-        packed::wait_copies<0>();
+        if constexpr (VEC)
+            wait_step<RING, S::PER, LOADS>();
+        else
+            packed::wait_copies<0>();
         x.start(s + RING - 1);
-        load8<VEC>(row, 32 * (s + AHEAD - 1) + 8 * (lane >> 4), p.hidden, w[(K + AHEAD - 1) % AHEAD]);
+        load(s + RING - 1, w[(K + RING - 1) % RING]);
+        __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
+        if (VEC && 32 * s + 8 * (lane >> 4) >= p.hidden)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[K][e] = 0.0f;
         bf16x8 a[3];
         split8(w[K], a);
         const __bf16* xs = lds + K * S::STEP;
@@ -255,20 +305,19 @@ __global__ __launch_bounds__(512, 2) void few_logits_kernel(FewLogits p) {
             if (lane < 16) red[wave * (16 * NB) + 16 * j + lane] = make_float2(m, s);
         }
         __syncthreads();
-        if (tid < 16 * NB) {
+        for (int t = tid; t < 16 * NB; t += blockDim.x) {
             float m = -__builtin_inff(), s = 0.0f;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) m = fmaxf(m, red[q * (16 * NB) + tid].x);
+            for (int q = 0; q < waves; ++q) m = fmaxf(m, red[q * (16 * NB) + t].x);
             const float at = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const float2 a = red[q * (16 * NB) + tid];
+            for (int q = 0; q < waves; ++q) {
+                const float2 a = red[q * (16 * NB) + t];
                 s += a.y * __builtin_amdgcn_exp2f((a.x - at) * LOG2E);
             }
-            p.part[(size_t)blockIdx.x * p.pitch + tid] = make_float2(m, s);
+            p.part[(size_t)blockIdx.x * p.pitch + t] = make_float2(m, s);
         }
     } else {
-        constexpr int PITCH = 36, STEPS_T = (NB + 1) / 2;
+        if (v0 >= p.blocks_v * 16) return;
+        constexpr int STEPS_T = (NB + 1) / 2;
         float* turn = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
         f32x4 db = {};
 #pragma unroll
@@ -293,7 +342,7 @@ __global__ __launch_bounds__(512, 2) void few_logits_kernel(FewLogits p) {
                     bf16x4 f[3];
                     split3_4(g, f[0], f[1], f[2]);
                     __bf16* to = p.g_rows + ((size_t)(v0 >> 5) * NB + j) * (3 * FRAG) +
-                                 (((wave & 1) * 2 + (lane >> 5)) * 16 + (lane & 15)) * 8 + 4 * ((lane >> 4) & 1);
+                                 ((((v0 >> 4) & 1) * 2 + (lane >> 5)) * 16 + (lane & 15)) * 8 + 4 * ((lane >> 4) & 1);
 #pragma unroll
                     for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x4*>(to + q * FRAG) = f[q];
                 }
@@ -333,11 +382,12 @@ struct FewDx {
     float* part;                    // [slice][16·NB][hidden]
 };
 
-// A workgroup: 256 columns of W (a wave 32) over a slice of the vocabulary.
-template <int NB, typename TW>
+// A workgroup: 256 columns of W over a slice of the vocabulary; a wave 32 of them, block i the columns 2·n + i, so that a
+// lane's two blocks come with one load a row (PAIR: rows of pairs).
+template <int NB, typename TW, bool PAIR>
 __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 3, RING = 4;
-    typedef Stream<NB, 8, RING> S;
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 3, LOADS = PAIR ? 8 : 16;
+    typedef Stream<3 * NB, 8, RING> S;
     __shared__ __attribute__((aligned(16))) __bf16 lds[RING * S::STEP];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = blockIdx.y * p.per, steps = min(p.per, p.steps - first);
@@ -346,30 +396,41 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
     const S g(p.g_rows + (size_t)first * S::STEP, lds, wave, lane, steps);
     int col[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) col[i] = min(h0 + 16 * i + (lane & 15), p.hidden - 1);
+    for (int i = 0; i < 2; ++i) col[i] = min(h0 + 2 * (lane & 15) + i, p.hidden - (PAIR ? 2 - i : 1));
     // Rows behind the vocabulary read its last: G is zero there.
     auto load = [&](int s, float (&w)[2][8]) {
         const int v = 32 * (first + min(s, steps - 1)) + 8 * (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[i][e] = (float)W[(size_t)min(v + e, p.vocab - 1) * p.hidden + col[i]];
+        for (int e = 0; e < 8; ++e) {
+            const TW* at = W + (size_t)min(v + e, p.vocab - 1) * p.hidden;
+            if constexpr (PAIR) {
+                typedef TW Pair __attribute__((ext_vector_type(2)));
+                const Pair both = *reinterpret_cast<const Pair*>(at + col[0]);
+                w[0][e] = (float)both[0];
+                w[1][e] = (float)both[1];
+            } else {
+                w[0][e] = (float)at[col[0]];
+                w[1][e] = (float)at[col[1]];
+            }
+        }
     };
-    float w[AHEAD][2][8];
+    float w[RING][2][8];
     f32x4 acc[2][NB];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{};
 #pragma unroll
-    for (int k = 0; k < RING - 1; ++k) g.start(k);
-#pragma unroll
-    for (int k = 0; k < AHEAD - 1; ++k) load(k, w[k]);
+    for (int k = 0; k < RING - 1; ++k) {
+        g.start(k);
+        load(k, w[k]);
+    }
     auto step = [&](int s, auto slot) {
         constexpr int K = decltype(slot)::value;
-        packed::wait_copies<0>();
+        wait_step<RING, S::PER, LOADS>();
         g.start(s + RING - 1);
-        load(s + AHEAD - 1, w[(K + AHEAD - 1) % AHEAD]);
+        load(s + RING - 1, w[(K + RING - 1) % RING]);
+        __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
         bf16x8 a[2][3];
         split8(w[K][0], a[0]);
         split8(w[K][1], a[1]);
@@ -394,10 +455,10 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
     for (int j = 0; j < NB; ++j) {
         float* to = p.part + ((size_t)blockIdx.y * (16 * NB) + 16 * j + (lane & 15)) * p.hidden;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int h = h0 + 16 * i + 4 * (lane >> 4) + e;
+            for (int i = 0; i < 2; ++i) {
+                const int h = h0 + 2 * (4 * (lane >> 4) + e) + i;
                 if (h < p.hidden) to[h] = acc[i][j][e];
             }
     }
@@ -428,108 +489,157 @@ __global__ __launch_bounds__(256) void few_dx_sum_kernel(const float* __restrict
 struct FewDw {
     const __bf16 *x_cols, *g_cols;
     const unsigned* words;
-    int hidden, vocab;
+    int hidden, vocab, blocks_v;
     float scale;
     float* dW;
 };
 
-// A wave: 16 rows of dW, their G in registers, all blocks of 16 columns one after another.
+// A wave: 16 rows of dW, their G in registers, HB blocks of 16 columns at a time. A chunk's x comes through LDS, its dW to
+// registers, both started while the chunk before is computed.
 template <int STEPS_T, bool VEC>
-__global__ __launch_bounds__(256) void few_dw_kernel(FewDw p) {
+__global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
     if (p.words[WORD_COUNT] == 0) return;
-    constexpr int FETCH = 4;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, vb = blockIdx.x * 4 + wave;
-    const int v = 16 * vb + (lane & 15), blocks = (p.hidden + 15) / 16;
-    if (16 * vb >= p.vocab) return;
+    constexpr int HB = STEPS_T == 1 ? 8 : 4;
+    typedef Stream<3 * STEPS_T * HB, 4, 2> S;
+    __shared__ __attribute__((aligned(16))) __bf16 lds[2 * S::STEP];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, vb = blockIdx.x * (int)(blockDim.x >> 6) + wave;
+    const int v = 16 * vb + (lane & 15), chunks = (p.hidden + 16 * HB - 1) / (16 * HB);
+    const bool live = v < p.vocab;
     bf16x8 g[STEPS_T][3];
 #pragma unroll
     for (int s = 0; s < STEPS_T; ++s)
 #pragma unroll
-        for (int q = 0; q < 3; ++q) g[s][q] = fragment(p.g_cols + (((size_t)vb * STEPS_T + s) * 3 + q) * FRAG, lane);
+        for (int q = 0; q < 3; ++q)
+            g[s][q] = fragment(p.g_cols + (((size_t)min(vb, p.blocks_v - 1) * STEPS_T + s) * 3 + q) * FRAG, lane);
     float* row = p.dW + (size_t)min(v, p.vocab - 1) * p.hidden;
-    const bool live = v < p.vocab;
-    auto fetch = [&](int hb) {
-        const int h = 16 * min(hb, blocks - 1) + 4 * (lane >> 4);
+    const S x(p.x_cols, lds, wave, lane, chunks);
+    auto fetch = [&](int chunk, int k) {
+        const int h = 16 * (chunk * HB + k) + 4 * (lane >> 4);
         f32x4 o = {};
         if constexpr (VEC) {
-            o = *reinterpret_cast<const f32x4*>(row + h);
+            if (h < p.hidden) o = *reinterpret_cast<const f32x4*>(row + h);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = row[min(h + e, p.hidden - 1)];
+            for (int e = 0; e < 4; ++e)
+                if (h + e < p.hidden) o[e] = row[h + e];
         }
         return o;
     };
-    f32x4 old[FETCH];
+    f32x4 next[HB];
+    x.start_once(0, wave);
 #pragma unroll
-    for (int k = 0; k < FETCH; ++k) old[k] = fetch(k);
-    for (int hb = 0; hb < blocks; hb += FETCH)
+    for (int k = 0; k < HB; ++k) next[k] = fetch(0, k);
+    for (int c = 0; c < chunks; ++c) {
+        packed::wait_copies<0>();
+        f32x4 now[HB];
 #pragma unroll
-        for (int k = 0; k < FETCH; ++k) {
-            if (hb + k >= blocks) break;
-            const __bf16* xs = p.x_cols + (size_t)(hb + k) * STEPS_T * (3 * FRAG);
-            f32x4 c = {};
+        for (int k = 0; k < HB; ++k) now[k] = next[k];
+        if (c + 1 < chunks) {
+            x.start_once(c + 1, wave);
+#pragma unroll
+            for (int k = 0; k < HB; ++k) next[k] = fetch(c + 1, k);
+        }
+        const __bf16* xs = lds + (c & 1) * S::STEP;
+#pragma unroll
+        for (int k = 0; k < HB; ++k) {
+            f32x4 sum = {};
 #pragma unroll
             for (int s = 0; s < STEPS_T; ++s) {
                 bf16x8 a[3];
 #pragma unroll
-                for (int q = 0; q < 3; ++q) a[q] = fragment(xs + (s * 3 + q) * FRAG, lane);
-                mma<3>(a, g[s], c);
+                for (int q = 0; q < 3; ++q) a[q] = fragment(xs + ((k * STEPS_T + s) * 3 + q) * FRAG, lane);
+                mma<3>(a, g[s], sum);
             }
-            const f32x4 now = old[k] + c * p.scale;
-            old[k] = fetch(hb + k + FETCH);
-            const int h = 16 * (hb + k) + 4 * (lane >> 4);
+            now[k] += sum * p.scale;
+            const int h = 16 * (c * HB + k) + 4 * (lane >> 4);
             if (!live) continue;
             if constexpr (VEC) {
-                *reinterpret_cast<f32x4*>(row + h) = now;
+                if (h < p.hidden) *reinterpret_cast<f32x4*>(row + h) = now[k];
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (h + e < p.hidden) row[h + e] = now[e];
+                    if (h + e < p.hidden) row[h + e] = now[k][e];
             }
         }
+    }
 }
 
 // ------------------------------------------------------------------------------------------ launches
 
-int blocks_of(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
+// Whether W's rows take 16-byte loads; without, the kernels of 8 blocks serve every number of rows.
+bool aligned_table(const VocabArgs& a) {
+    return a.hidden % 8 == 0 && ((a.W16 ? (uintptr_t)a.W16 : (uintptr_t)a.W) & 15u) == 0;
+}
+int blocks_of(const VocabArgs& a) {
+    const int b = (a.rows + 15) / 16;
+    return !aligned_table(a) || b == 7 ? 8 : b;
+}
 
-template <int NB, bool GRAD>
-void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p) {
-    const dim3 grid((a.vocab + FEW_V - 1) / FEW_V), block(512);
-    const bool vec = a.hidden % 8 == 0 && ((uintptr_t)p.W & 15u) == 0;
+// Waves of a workgroup of few_logits and few_dw, a block of 16 rows of W each: as few as take the table in the rounds that
+// 16 would take, one workgroup a CU, and 4 at least.
+int waves_of(const laya_ctx* ctx, int blocks_v) {
+    const int rounds = (blocks_v + 16 * ctx->cu_count - 1) / (16 * ctx->cu_count);
+    return std::max(4, (blocks_v + rounds * ctx->cu_count - 1) / (rounds * ctx->cu_count));
+}
+
+// f(the number of blocks as a constant).
+template <class F> void with_blocks(int nb, F&& f) {
+    if (nb == 1) f(std::integral_constant<int, 1>());
+    else if (nb == 2) f(std::integral_constant<int, 2>());
+    else if (nb == 3) f(std::integral_constant<int, 3>());
+    else if (nb == 4) f(std::integral_constant<int, 4>());
+    else if (nb == 5) f(std::integral_constant<int, 5>());
+    else if (nb == 6) f(std::integral_constant<int, 6>());
+    else f(std::integral_constant<int, 8>());
+}
+
+template <bool GRAD>
+void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p, int nb, int waves) {
+    const dim3 grid((p.blocks_v + waves - 1) / waves), block(64 * waves);
     ProfileScope scope(ctx, "vocab_few_logits", 2.0 * a.rows * a.hidden * a.vocab,
                        (a.W16 ? 2.0 : 4.0) * a.hidden * a.vocab);
-    if (a.W16 && vec)
-        LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD>), grid, block, 0, ctx->stream, p);
-    else if (a.W16)
-        LAYA_LAUNCH((few_logits_kernel<NB, __bf16, false, GRAD>), grid, block, 0, ctx->stream, p);
-    else if (vec)
-        LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD>), grid, block, 0, ctx->stream, p);
-    else
-        LAYA_LAUNCH((few_logits_kernel<NB, float, false, GRAD>), grid, block, 0, ctx->stream, p);
+    if (!aligned_table(a)) {
+        if (a.W16)
+            LAYA_LAUNCH((few_logits_kernel<8, __bf16, false, GRAD, 4>), grid, block, 0, ctx->stream, p);
+        else
+            LAYA_LAUNCH((few_logits_kernel<8, float, false, GRAD, 4>), grid, block, 0, ctx->stream, p);
+    } else {
+        with_blocks(nb, [&](auto n) {
+            constexpr int NB = decltype(n)::value;
+            if (a.W16 && waves >= 8)
+                LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, 8>), grid, block, 0, ctx->stream, p);
+            else if (a.W16)
+                LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, 4>), grid, block, 0, ctx->stream, p);
+            else if (waves >= 8)
+                LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, 8>), grid, block, 0, ctx->stream, p);
+            else
+                LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, 4>), grid, block, 0, ctx->stream, p);
+        });
+    }
     check_launch("few_logits_kernel");
 }
-template <bool GRAD>
-void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p, int nb) {
-    if (nb == 1) launch_logits<1, GRAD>(ctx, a, p);
-    else if (nb == 2) launch_logits<2, GRAD>(ctx, a, p);
-    else if (nb == 4) launch_logits<4, GRAD>(ctx, a, p);
-    else launch_logits<8, GRAD>(ctx, a, p);
-}
 
-template <int NB>
-void launch_dx(laya_ctx* ctx, const VocabArgs& a, const FewDx& p, int slices) {
+void launch_dx(laya_ctx* ctx, const VocabArgs& a, const FewDx& p, int slices, int nb) {
     const dim3 grid((a.hidden + 255) / 256, slices), block(512);
-    if (a.W16)
-        LAYA_LAUNCH((few_dx_kernel<NB, __bf16>), grid, block, 0, ctx->stream, p);
-    else
-        LAYA_LAUNCH((few_dx_kernel<NB, float>), grid, block, 0, ctx->stream, p);
+    ProfileScope scope(ctx, "vocab_few_dx", 2.0 * a.rows * a.hidden * a.vocab,
+                       (a.W16 ? 2.0 : 4.0) * a.hidden * a.vocab);
+    with_blocks(nb, [&](auto n) {
+        constexpr int NB = decltype(n)::value;
+        if (a.W16 && aligned_table(a))
+            LAYA_LAUNCH((few_dx_kernel<NB, __bf16, true>), grid, block, 0, ctx->stream, p);
+        else if (a.W16)
+            LAYA_LAUNCH((few_dx_kernel<NB, __bf16, false>), grid, block, 0, ctx->stream, p);
+        else if (aligned_table(a))
+            LAYA_LAUNCH((few_dx_kernel<NB, float, true>), grid, block, 0, ctx->stream, p);
+        else
+            LAYA_LAUNCH((few_dx_kernel<NB, float, false>), grid, block, 0, ctx->stream, p);
+    });
     check_launch("few_dx_kernel");
 }
 
 template <int STEPS_T>
-void launch_dw(laya_ctx* ctx, const VocabArgs& a, const FewDw& p) {
-    const dim3 grid((a.vocab + 63) / 64), block(256);
+void launch_dw(laya_ctx* ctx, const VocabArgs& a, const FewDw& p, int waves) {
+    const dim3 grid((p.blocks_v + waves - 1) / waves), block(64 * waves);
     ProfileScope scope(ctx, "vocab_few_dw", 2.0 * a.rows * a.hidden * a.vocab, 8.0 * a.hidden * a.vocab);
     if (a.hidden % 16 == 0 && ((uintptr_t)p.dW & 15u) == 0)
         LAYA_LAUNCH((few_dw_kernel<STEPS_T, true>), grid, block, 0, ctx->stream, p);
@@ -541,8 +651,9 @@ void launch_dw(laya_ctx* ctx, const VocabArgs& a, const FewDw& p) {
 }  // namespace
 
 void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count) {
-    const int nb = blocks_of(a.rows), pitch = 16 * nb, steps = packed::steps_of(a.hidden);
-    const int tiles = (a.vocab + FEW_V - 1) / FEW_V;
+    const int nb = blocks_of(a), pitch = 16 * nb, steps = packed::steps_of(a.hidden);
+    const int blocks_v = 2 * packed::steps_of(a.vocab), waves = waves_of(ctx, blocks_v);
+    const int tiles = (blocks_v + waves - 1) / waves;
     unsigned* words;
     int* row_of;
     __bf16* x_rows;
@@ -565,15 +676,16 @@ void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* ls
     p.hidden = a.hidden;
     p.vocab = a.vocab;
     p.steps = steps;
+    p.blocks_v = blocks_v;
     p.part = part;
     p.pitch = pitch;
-    launch_logits<false>(ctx, a, p, nb);
+    launch_logits<false>(ctx, a, p, nb, waves);
     vocab_merge(ctx, a, part, pitch, tiles, words, row_of, row_loss, lse, loss);
 }
 
 void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {
-    const int nb = blocks_of(a.rows), steps_t = (nb + 1) / 2, steps = packed::steps_of(a.hidden);
-    const int tiles = (a.vocab + FEW_V - 1) / FEW_V, steps_v = packed::steps_of(a.vocab);
+    const int nb = blocks_of(a), steps_t = (nb + 1) / 2, steps = packed::steps_of(a.hidden);
+    const int steps_v = packed::steps_of(a.vocab), blocks_v = 2 * steps_v, waves = waves_of(ctx, blocks_v);
     // Slices of the vocabulary, so that few_dx's workgroups are about as many as the chip's CUs.
     const int across = (a.hidden + 255) / 256;
     const int per = std::max(4, (steps_v + std::max(1, ctx->cu_count / across) - 1) / std::max(1, ctx->cu_count / across));
@@ -587,9 +699,9 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
         ws.take(row_of, a.rows);
         ws.take(place, a.rows);
         ws.take(x_rows, (size_t)steps * nb * 3 * FRAG);
-        ws.take(x_cols, (size_t)2 * steps * steps_t * 3 * FRAG);
-        ws.take(g_rows, (size_t)tiles * (FEW_V / 32) * nb * 3 * FRAG);
-        ws.take(g_cols, (size_t)tiles * (FEW_V / 16) * steps_t * 3 * FRAG);
+        ws.take(x_cols, (size_t)(2 * steps + 6) * steps_t * 3 * FRAG);  // few_dw reads whole chunks of up to 8 blocks
+        ws.take(g_rows, (size_t)steps_v * nb * 3 * FRAG);
+        ws.take(g_cols, (size_t)blocks_v * steps_t * 3 * FRAG);
         ws.take(part, (size_t)slices * 16 * nb * a.hidden);
     });
     const Prepare prep{a.x, a.row_weights, a.targets, a.rows, a.hidden, a.vocab, nb, x_rows, x_cols,
@@ -604,6 +716,7 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
     p.hidden = a.hidden;
     p.vocab = a.vocab;
     p.steps = steps;
+    p.blocks_v = blocks_v;
     p.row_of = row_of;
     p.targets = a.targets;
     p.lse = lse;
@@ -612,26 +725,20 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
     p.g_cols = g_cols;
     p.db = db;
     p.scale = a.scale;
-    launch_logits<true>(ctx, a, p, nb);
+    launch_logits<true>(ctx, a, p, nb, waves);
     if (dx) {
         const FewDx q{p.W, g_rows, a.hidden, a.vocab, steps_v, per, part};
-        {
-            ProfileScope scope(ctx, "vocab_few_dx", 2.0 * a.rows * a.hidden * a.vocab,
-                               (a.W16 ? 2.0 : 4.0) * a.hidden * a.vocab);
-            if (nb == 1) launch_dx<1>(ctx, a, q, slices);
-            else if (nb == 2) launch_dx<2>(ctx, a, q, slices);
-            else if (nb == 4) launch_dx<4>(ctx, a, q, slices);
-            else launch_dx<8>(ctx, a, q, slices);
-        }
+        launch_dx(ctx, a, q, slices, nb);
         LAYA_LAUNCH(few_dx_sum_kernel, dim3((a.hidden + 255) / 256, a.rows), dim3(256), 0, ctx->stream, part, slices,
                     16 * nb, place, a.row_weights, a.scale, a.hidden, dx);
         check_launch("few_dx_sum_kernel");
     }
     if (dW) {
-        const FewDw q{x_cols, g_cols, words, a.hidden, a.vocab, a.scale, dW};
-        if (steps_t == 1) launch_dw<1>(ctx, a, q);
-        else if (steps_t == 2) launch_dw<2>(ctx, a, q);
-        else launch_dw<4>(ctx, a, q);
+        const FewDw q{x_cols, g_cols, words, a.hidden, a.vocab, blocks_v, a.scale, dW};
+        if (steps_t == 1) launch_dw<1>(ctx, a, q, waves);
+        else if (steps_t == 2) launch_dw<2>(ctx, a, q, waves);
+        else if (steps_t == 3) launch_dw<3>(ctx, a, q, waves);
+        else launch_dw<4>(ctx, a, q, waves);
     }
 }
 
