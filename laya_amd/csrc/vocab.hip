@@ -324,7 +324,27 @@ __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restri
     const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, count = (int)words[WORD_COUNT];
     if (j < count) {
         const int r = row_of[j], y = targets[r];
-        double z = 0.0;
+        // The target's row first: its loads are under way while the tiles' arrive.
+        const float* xr = x + (size_t)r * hidden;
+        const TW* wr = W + (size_t)y * hidden;
+        double z = 0.0, z1 = 0.0;
+        int k0 = lane;
+#pragma unroll 2
+        for (; k0 + 448 < hidden; k0 += 512) {
+            float xv[8], wv[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                xv[q] = xr[k0 + 64 * q];
+                wv[q] = (float)wr[k0 + 64 * q];
+            }
+#pragma unroll
+            for (int q = 0; q < 8; q += 2) {
+                z += (double)xv[q] * wv[q];
+                z1 += (double)xv[q + 1] * wv[q + 1];
+            }
+        }
+#pragma unroll 4
+        for (; k0 < hidden; k0 += 64) z += (double)xr[k0] * (double)(float)wr[k0];
         // Each lane's tiles, four at a time: the maximum and the sum so far.
         float m = -__builtin_inff(), s = 0.0f;
         for (int k = lane; k < tiles; k += 256) {
@@ -339,14 +359,12 @@ __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restri
             for (int q = 0; q < 4; ++q) s = fmaf(a[q].y, __builtin_amdgcn_exp2f((a[q].x - at) * LOG2E), s);
             m = top;
         }
-        for (int k = lane; k < hidden; k += 64)
-            z += (double)x[(size_t)r * hidden + k] * (double)(float)W[(size_t)y * hidden + k];
         float top = m;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         const float at = top == -__builtin_inff() ? 0.0f : top;
         const double sum = wave_sum_d((double)(s * __builtin_amdgcn_exp2f((m - at) * LOG2E)));
-        z = wave_sum_d(z);
+        z = wave_sum_d(z + z1);
         if (lane == 0) {
             const double l = (double)top + log(sum);
             lse[r] = (float)l;

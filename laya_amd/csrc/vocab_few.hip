@@ -1,13 +1,15 @@
 // The vocabulary cross entropy of up to 128 rows, where the table's own bytes are the cost: every kernel reads W (or
 // moves dW) once, straight from memory, and splits it in registers.
 //
-// The products are exact three-piece bf16 splits (split.hpp): six matrix products for one, but no scale, and so no pass
-// over W to find one; up to 128 rows their time hides behind the table's. bf16 weights are one piece, three products.
+// The products are two-piece fp16 products (split.hpp) as the large ones, three matrix products each, but W is split as it
+// streams by, so its scale is found on the way: a wave scales its 16 rows from the largest magnitude so far, with four
+// bits to spare, and when a value would leave fp16's range it takes a new scale and brings its sums to it (a power of
+// two, so exactly), as the running maximum of a softmax is handled. bf16 weights are one piece, two products.
 //   few_prepare   the labelled rows' x as fragments, rows t over h and (weighted) rows h over t
 //   few_logits    z = W·xᵀ, a wave 16 rows of W (its 8 k of a lane are two 16-byte loads); statistics, or G in both orders
-//   few_dx        dxᵀ = Wᵀ·Gᵀ over slices of the vocabulary, a lane's 8 k eight loads down W's column
+//   few_dx        dxᵀ = Wᵀ·Gᵀ over slices of the vocabulary, a lane's 8 k eight loads down W's columns
 //   few_dw        dWᵀ += xᵀ·G, a lane four neighbours of one row of dW
-// Fragments are 16 rows x 32 k of v_mfma_f32_16x16x32_bf16, [k / 8][row][8 k], three planes one after another.
+// Fragments are 16 rows x 32 k of v_mfma_f32_16x16x32_f16, [k / 8][row][8 k], the two planes one after another.
 #include "elementwise.hpp"
 #include "packed.hpp"
 #include "vocab.hpp"
@@ -18,75 +20,102 @@ namespace {
 using packed::FRAG;
 using packed::lds_byte;
 
-__device__ __forceinline__ void split8(const float (&v)[8], bf16x8 (&p)[3]) {
-    bf16x4 a[3], b[3];
-    split3_4(f32x4{v[0], v[1], v[2], v[3]}, a[0], a[1], a[2]);
-    split3_4(f32x4{v[4], v[5], v[6], v[7]}, b[0], b[1], b[2]);
+constexpr int PLANES = 2, BLOCK = PLANES * FRAG;  // a fragment's fp16 values, both planes
+constexpr int G_SCALE = 14;                       // |G| ≤ 1
+
+__device__ __forceinline__ void split8(const float (&v)[8], float sc, f16x8 (&p)[2]) {
+    f16x4 a[2], b[2];
+    split2h_4(f32x4{v[0], v[1], v[2], v[3]}, sc, a[0], a[1]);
+    split2h_4(f32x4{v[4], v[5], v[6], v[7]}, sc, b[0], b[1]);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) p[k] = __builtin_shufflevector(a[k], b[k], 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int k = 0; k < 2; ++k) p[k] = __builtin_shufflevector(a[k], b[k], 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// c += a·b of three-piece operands (PA = 1: a is one piece), smallest products first.
+// c += a·b of two-piece operands (PA = 1: a is one piece), smallest products first.
 template <int PA>
-__device__ __forceinline__ void mma(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x4& c) {
-    if constexpr (PA == 3) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[0], c, 0, 0, 0);
-    } else {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], c, 0, 0, 0);
-    }
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[1], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], c, 0, 0, 0);
+__device__ __forceinline__ void mma(const f16x8 (&a)[2], const f16x8 (&b)[2], f32x4& c) {
+    if constexpr (PA == 2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], b[0], c, 0, 0, 0);
 }
-__device__ __forceinline__ bf16x8 fragment(const __bf16* at, int lane) {
-    return *reinterpret_cast<const bf16x8*>(at + lane * 8);
+__device__ __forceinline__ f16x8 fragment(const _Float16* at, int lane) {
+    return *reinterpret_cast<const f16x8*>(at + lane * 8);
 }
 
-// The labelled rows in order, by every workgroup for itself: row_of[j] (LDS) and their number. Rows ≤ VOCAB_FEW ≤ 256.
+// The labelled rows in order, by every workgroup for itself: row_of[j] (LDS) and their number. VOCAB_FEW ≤ 128 rows.
 __device__ __forceinline__ int list_rows(const int* targets, int rows, int vocab, int* row_of, int& bad) {
-    __shared__ int wave_count[4], wave_bad[4];
+    __shared__ int wave_count[2], wave_bad[2];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int y = tid < rows ? targets[tid] : LAYA_NO_LABEL;
-    const bool has = tid < 256 && y >= 0 && y < vocab;
-    const unsigned long long m = __ballot(has), wrong = __ballot(tid < 256 && !has && y != LAYA_NO_LABEL);
-    if (lane == 0 && wave < 4) {
+    const bool has = y >= 0 && y < vocab;
+    const unsigned long long m = __ballot(has), wrong = __ballot(!has && y != LAYA_NO_LABEL);
+    if (lane == 0 && wave < 2) {
         wave_count[wave] = __popcll(m);
         wave_bad[wave] = __popcll(wrong);
     }
     __syncthreads();
-    int before = 0, count = 0;
-    bad = 0;
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += wave_count[w];
-        count += wave_count[w];
-        bad += wave_bad[w];
-    }
-    if (has) row_of[before + __popcll(m & ((1ull << lane) - 1))] = tid;
+    bad = wave_bad[0] + wave_bad[1];
+    if (has) row_of[(wave ? wave_count[0] : 0) + __popcll(m & ((1ull << lane) - 1))] = tid;
     __syncthreads();
-    return count;
+    return wave_count[0] + wave_count[1];
 }
 
 struct Prepare {
     const float *x, *weights;
     const int* targets;
     int rows, hidden, vocab, blocks_t;  // blocks_t: blocks of 16 rows, padded
-    __bf16* x_rows;                     // [k step][block of t][3][FRAG]
-    __bf16* x_cols;                     // [block of 16 h][step of 32 t][3][FRAG], weighted (null: not wanted)
+    _Float16* x_rows;                   // [k step][block of t][2][FRAG], rows scaled by 2^exps[t]
+    _Float16* x_cols;                   // [block of 16 h][step of 32 t][2][FRAG], weighted (null: not wanted)
+    int* exps;
     int *row_of, *place, *bad_count;
     unsigned* words;
     float *row_loss, *lse;              // of the forward (null in the backward)
 };
 
-// One workgroup a step of 32 columns of x.
-__global__ __launch_bounds__(256) void few_prepare_kernel(Prepare p) {
-    __shared__ int row_of[256];
-    __shared__ float tile[32][33];
+// One workgroup a step of 32 columns of x; each finds the rows' scales for itself. VEC: rows of float4s.
+template <bool VEC>
+__global__ __launch_bounds__(1024) void few_prepare_kernel(Prepare p) {
+    __shared__ int row_of[VOCAB_FEW], row_exp[VOCAB_FEW];
+    __shared__ float tile[VOCAB_FEW][33];
+    __shared__ unsigned whole;
     const int tid = threadIdx.x, step = blockIdx.x;
     int bad;
+    if (tid == 0) whole = 0;
     const int count = list_rows(p.targets, p.rows, p.vocab, row_of, bad);
+    {  // thread t four columns of row t / 8 of this step
+        const int j = tid >> 3, c = 32 * step + 4 * (tid & 7);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            tile[j][4 * (tid & 7) + i] =
+                j < count && c + i < p.hidden ? p.x[(size_t)row_of[j] * p.hidden + c + i] : 0.0f;
+    }
+    for (int j = tid >> 4; j < 16 * p.blocks_t; j += 64) {  // 16 threads a row
+        unsigned m = 0;
+        if (j < count) {
+            const float* row = p.x + (size_t)row_of[j] * p.hidden;
+            if constexpr (VEC) {
+#pragma unroll 8
+                for (int c = 4 * (tid & 15); c < p.hidden; c += 64)
+                    m = max(m, amax_bits4(*reinterpret_cast<const f32x4*>(row + c)));
+            } else {
+                for (int c = tid & 15; c < p.hidden; c += 16) m = max(m, amax_bits(row[c]));
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+        if ((tid & 15) == 0) {
+            const int e = pair_scale_exp(m);
+            row_exp[j] = e;
+            if (step == 0) p.exps[j] = e;
+            if (j < count) {
+                const float w = p.weights ? fabsf(p.weights[row_of[j]]) : 1.0f;
+                atomicMax(&whole, amax_bits(__builtin_bit_cast(float, m) * w));
+            }
+        }
+    }
+    __syncthreads();
     if (step == 0) {
-        if (tid < WORDS) p.words[tid] = tid == WORD_COUNT ? count : tid == WORD_BAD ? bad : 0;
+        if (tid < WORDS)
+            p.words[tid] = tid == WORD_COUNT ? count : tid == WORD_BAD ? bad : tid == WORD_WX ? whole : 0;
         if (tid == 0 && p.bad_count) *p.bad_count = bad;
         if (tid < p.rows) {
             const int y = p.targets[tid];
@@ -99,39 +128,30 @@ __global__ __launch_bounds__(256) void few_prepare_kernel(Prepare p) {
             if (p.place) p.place[row_of[tid]] = tid;
         }
     }
-    const int steps_t = (p.blocks_t + 1) / 2;
-    for (int s = 0; s < steps_t; ++s) {  // 32 rows of x at a time: thread t four columns of row t / 8
-        const int j = 32 * s + (tid >> 3), c = 32 * step + 4 * (tid & 7);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            tile[tid >> 3][4 * (tid & 7) + i] =
-                j < count && c + i < p.hidden ? p.x[(size_t)row_of[j] * p.hidden + c + i] : 0.0f;
-        __syncthreads();
-        if (tid >= 128) continue;  // unit tid: row r, octet o
-        float v[8];
-        bf16x8 f[3];
-        const int r = tid >> 2, o = tid & 3;
+    const int o = tid & 3, steps_t = (p.blocks_t + 1) / 2;
+    float v[8];
+    f16x8 f[2];
+    if (tid < 512) {  // row r over h, octet o
+        const int r = tid >> 2, tb = r >> 4;
+        if (tb >= p.blocks_t) return;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[r][8 * o + i];
-        split8(v, f);
-        const int tb = 2 * s + (r >> 4);
-        if (tb < p.blocks_t) {
-            __bf16* to = p.x_rows + ((size_t)step * p.blocks_t + tb) * (3 * FRAG) + (o * 16 + (r & 15)) * 8;
+        split8(v, exp2_int(row_exp[r]), f);
+        _Float16* to = p.x_rows + ((size_t)step * p.blocks_t + tb) * BLOCK + (o * 16 + (r & 15)) * 8;
 #pragma unroll
-            for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(to + k * FRAG) = f[k];
+        for (int k = 0; k < 2; ++k) *reinterpret_cast<f16x8*>(to + k * FRAG) = f[k];
+    } else if (p.x_cols) {  // column 32·step + r over t, octet o of step s
+        const int r = ((tid - 512) >> 2) & 31, s = (tid - 512) >> 7;
+        if (s >= steps_t) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = 32 * s + 8 * o + i;
+            v[i] = t < count ? tile[t][r] * (p.weights ? p.weights[row_of[t]] : 1.0f) : 0.0f;
         }
-        if (p.x_cols) {  // row r of this side: column 32·step + r of x, over t
+        split8(v, exp2_int(pair_scale_exp(whole)), f);
+        _Float16* to = p.x_cols + ((size_t)(2 * step + (r >> 4)) * steps_t + s) * BLOCK + (o * 16 + (r & 15)) * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = 32 * s + 8 * o + i;
-                v[i] = t < count ? tile[8 * o + i][r] * (p.weights ? p.weights[row_of[t]] : 1.0f) : 0.0f;
-            }
-            split8(v, f);
-            __bf16* to = p.x_cols + ((size_t)(2 * step + (r >> 4)) * steps_t + s) * (3 * FRAG) + (o * 16 + (r & 15)) * 8;
-#pragma unroll
-            for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(to + k * FRAG) = f[k];
-        }
+        for (int k = 0; k < 2; ++k) *reinterpret_cast<f16x8*>(to + k * FRAG) = f[k];
     }
 }
 
@@ -142,10 +162,10 @@ __global__ __launch_bounds__(256) void few_prepare_kernel(Prepare p) {
 template <int KB, int WAVES, int RING>
 struct Stream {
     static constexpr int PER = (KB + WAVES - 1) / WAVES, STEP = KB * FRAG;
-    const __bf16* from;
+    const _Float16* from;
     unsigned lds0;
     int chunk[PER], last;
-    __device__ __forceinline__ Stream(const __bf16* data, const __bf16* lds, int wave, int lane, int steps)
+    __device__ __forceinline__ Stream(const _Float16* data, const _Float16* lds, int wave, int lane, int steps)
         : from(data + lane * 8), lds0(lds_byte(lds)), last(steps - 1) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) chunk[k] = __builtin_amdgcn_readfirstlane(min(wave + k * (int)(blockDim.x >> 6), KB - 1));
@@ -186,8 +206,9 @@ __device__ __forceinline__ void wait_step() {
 struct FewLogits {
     const void* W;
     const float* bias;
-    const __bf16* x_rows;
-    const unsigned* words;
+    const _Float16* x_rows;
+    const int* exps;
+    unsigned* words;
     int hidden, vocab, steps, blocks_v;  // blocks_v: blocks of 16 rows of W, an even number
     // Statistics:
     float2* part;            // [workgroup][pitch]
@@ -195,8 +216,8 @@ struct FewLogits {
     // G:
     const int *row_of, *targets;
     const float *lse, *weights;
-    __bf16* g_rows;          // [step of 32 v][block of t][3][FRAG]: rows t over v
-    __bf16* g_cols;          // [block of 16 v][step of 32 t][3][FRAG]: rows v over t
+    _Float16* g_rows;        // [step of 32 v][block of t][2][FRAG]: rows t over v
+    _Float16* g_cols;        // [block of 16 v][step of 32 t][2][FRAG]: rows v over t
     float* db;
     float scale;
 };
@@ -223,10 +244,10 @@ __device__ __forceinline__ void load8_always(const __bf16* row, int c, int K, fl
 // A workgroup is as many waves, WAVES at least, as spread the table's blocks of 16 rows evenly over the CUs.
 template <int NB, typename TW, bool VEC, bool GRAD, int WAVES>
 __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 3, LOADS = sizeof(TW) == 2 ? 1 : 2;
-    typedef Stream<3 * NB, WAVES, RING> S;
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = sizeof(TW) == 2 ? 1 : 2;
+    typedef Stream<2 * NB, WAVES, RING> S;
     constexpr int PITCH = 36, ROOM = GRAD ? 16 * 16 * PITCH * 2 : 16 * 16 * NB * 4;  // what the end needs
-    __shared__ __attribute__((aligned(16))) __bf16 lds[RING * S::STEP < ROOM ? ROOM : RING * S::STEP];
+    __shared__ __attribute__((aligned(16))) _Float16 lds[RING * S::STEP < ROOM ? ROOM : RING * S::STEP];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, waves = blockDim.x >> 6, steps = p.steps;
     const int v0 = (blockIdx.x * waves + wave) * 16;
     const TW* row = static_cast<const TW*>(p.W) + (size_t)min(v0 + (lane & 15), p.vocab - 1) * p.hidden;
@@ -239,6 +260,9 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
             load8<false>(row, c, p.hidden, w);
     };
     float w[RING][8];
+    int e = 126;           // of the wave's scale
+    float limit = 0.0f;    // magnitudes from here on need another
+    float top = 0.0f;      // the lane's largest
     f32x4 acc[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[j] = f32x4{};
@@ -260,14 +284,33 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
         if (VEC && 32 * s + 8 * (lane >> 4) >= p.hidden)
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[K][e] = 0.0f;
-        bf16x8 a[3];
-        split8(w[K], a);
-        const __bf16* xs = lds + K * S::STEP;
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(w[K][k]));
+        if (__any(m >= limit)) {  // a new scale (of infinities, none: they reach the sums as such)
+            unsigned bits = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) bits = max(bits, amax_bits(w[K][k]));
+            m = __builtin_bit_cast(float, bits);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o, 64));
+            const int to = min(e, pair_scale_exp(bits) - 3);
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], to - e);
+            e = to;
+            limit = exp2_int(min(15 - e, 127));
+        }
+        if (GRAD) top = fmaxf(top, m);
+        f16x8 a[2];
+        split8(w[K], exp2_int(max(e, -126)), a);
+        const _Float16* xs = lds + K * S::STEP;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            bf16x8 b[3];
+            f16x8 b[2];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) b[q] = fragment(xs + (3 * j + q) * FRAG, lane);
+            for (int q = 0; q < 2; ++q) b[q] = fragment(xs + (2 * j + q) * FRAG, lane);
             mma<PW>(a, b, acc[j]);
         }
     };
@@ -279,27 +322,26 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
     }
     packed::wait_copies<0>();
     const int count = (int)p.words[WORD_COUNT];
-    float b[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int v = v0 + 4 * (lane >> 4) + r;
-        b[r] = v < p.vocab ? (p.bias ? p.bias[v] : 0.0f) : -__builtin_inff();
+        const float b = v < p.vocab ? (p.bias ? p.bias[v] : 0.0f) : -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], -(e + p.exps[16 * j + (lane & 15)])) + b;
     }
     if constexpr (!GRAD) {
         float2* red = reinterpret_cast<float2*>(lds);  // [wave][16·NB]
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            float m = -__builtin_inff(), s = 0.0f, z[4];
+            float m = -__builtin_inff(), s = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                z[r] = acc[j][r] + b[r];
-                m = fmaxf(m, z[r]);
-            }
+            for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[j][r]);
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const float at = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((z[r] - at) * LOG2E);
+            for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[j][r] - at) * LOG2E);
             s += __shfl_xor(s, 16, 64);
             s += __shfl_xor(s, 32, 64);
             if (lane < 16) red[wave * (16 * NB) + 16 * j + lane] = make_float2(m, s);
@@ -316,6 +358,12 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
             p.part[(size_t)blockIdx.x * p.pitch + t] = make_float2(m, s);
         }
     } else {
+        __shared__ unsigned largest;
+        if (tid == 0) largest = 0;
+        __syncthreads();
+        atomicMax(&largest, __builtin_bit_cast(unsigned, top));
+        __syncthreads();
+        if (tid == 0) atomicMax(p.words + WORD_W, largest);
         if (v0 >= p.blocks_v * 16) return;
         constexpr int STEPS_T = (NB + 1) / 2;
         float* turn = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
@@ -333,31 +381,31 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
                     const int y = (live ? p.targets[r] : -1) - (v0 + 4 * (lane >> 4));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float q = __builtin_amdgcn_exp2f((acc[j][e] + b[e] - lse) * LOG2E);
+                        float q = __builtin_amdgcn_exp2f((acc[j][e] - lse) * LOG2E);
                         q -= y == e ? 1.0f : 0.0f;
-                        g[e] = live ? q : 0.0f;
+                        g[e] = live ? q * (float)(1 << G_SCALE) : 0.0f;
                     }
                     const float wt = live ? (p.weights ? p.weights[r] : 1.0f) : 0.0f;
                     db += live ? g * wt : f32x4{};
-                    bf16x4 f[3];
-                    split3_4(g, f[0], f[1], f[2]);
-                    __bf16* to = p.g_rows + ((size_t)(v0 >> 5) * NB + j) * (3 * FRAG) +
+                    f16x4 f[2];
+                    split2h_4(g, 1.0f, f[0], f[1]);
+                    _Float16* to = p.g_rows + ((size_t)(v0 >> 5) * NB + j) * BLOCK +
                                  ((((v0 >> 4) & 1) * 2 + (lane >> 5)) * 16 + (lane & 15)) * 8 + 4 * ((lane >> 4) & 1);
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x4*>(to + q * FRAG) = f[q];
+                    for (int q = 0; q < 2; ++q) *reinterpret_cast<f16x4*>(to + q * FRAG) = f[q];
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) turn[(4 * (lane >> 4) + e) * PITCH + 16 * jj + (lane & 15)] = g[e];
             }
             float v[8];
-            bf16x8 f[3];
+            f16x8 f[2];
             const float* at = turn + (lane & 15) * PITCH + 8 * (lane >> 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = at[e];
-            split8(v, f);
-            __bf16* to = p.g_cols + ((size_t)(v0 >> 4) * STEPS_T + ts) * (3 * FRAG) + lane * 8;
+            split8(v, 1.0f, f);
+            _Float16* to = p.g_cols + ((size_t)(v0 >> 4) * STEPS_T + ts) * BLOCK + lane * 8;
 #pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(to + q * FRAG) = f[q];
+            for (int q = 0; q < 2; ++q) *reinterpret_cast<f16x8*>(to + q * FRAG) = f[q];
         }
         if (p.db) {
 #pragma unroll
@@ -368,7 +416,7 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
             if ((lane & 15) == 0)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (v + e < p.vocab) p.db[v + e] += db[e] * p.scale;
+                    if (v + e < p.vocab) p.db[v + e] += db[e] * (1.0f / (1 << G_SCALE)) * p.scale;
         }
     }
 }
@@ -377,7 +425,8 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
 
 struct FewDx {
     const void* W;
-    const __bf16* g_rows;
+    const _Float16* g_rows;
+    const unsigned* words;
     int hidden, vocab, steps, per;  // steps of 32 v in all, and of a slice
     float* part;                    // [slice][16·NB][hidden]
 };
@@ -386,9 +435,9 @@ struct FewDx {
 // lane's two blocks come with one load a row (PAIR: rows of pairs).
 template <int NB, typename TW, bool PAIR>
 __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 3, LOADS = PAIR ? 8 : 16;
-    typedef Stream<3 * NB, 8, RING> S;
-    __shared__ __attribute__((aligned(16))) __bf16 lds[RING * S::STEP];
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = PAIR ? 8 : 16;
+    typedef Stream<2 * NB, 8, RING> S;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[RING * S::STEP];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = blockIdx.y * p.per, steps = min(p.per, p.steps - first);
     const int h0 = blockIdx.x * 256 + wave * 32;
@@ -414,6 +463,8 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
             }
         }
     };
+    const int ew = pair_scale_exp(p.words[WORD_W]);
+    const float sc = exp2_int(ew);
     float w[RING][2][8];
     f32x4 acc[2][NB];
 #pragma unroll
@@ -431,15 +482,15 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
         g.start(s + RING - 1);
         load(s + RING - 1, w[(K + RING - 1) % RING]);
         __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
-        bf16x8 a[2][3];
-        split8(w[K][0], a[0]);
-        split8(w[K][1], a[1]);
-        const __bf16* gs = lds + K * S::STEP;
+        f16x8 a[2][2];
+        split8(w[K][0], sc, a[0]);
+        split8(w[K][1], sc, a[1]);
+        const _Float16* gs = lds + K * S::STEP;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            bf16x8 b[3];
+            f16x8 b[2];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) b[q] = fragment(gs + (3 * j + q) * FRAG, lane);
+            for (int q = 0; q < 2; ++q) b[q] = fragment(gs + (2 * j + q) * FRAG, lane);
             mma<PW>(a[0], b, acc[0][j]);
             mma<PW>(a[1], b, acc[1][j]);
         }
@@ -459,7 +510,7 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int h = h0 + 2 * (4 * (lane >> 4) + e) + i;
-                if (h < p.hidden) to[h] = acc[i][j][e];
+                if (h < p.hidden) to[h] = __builtin_amdgcn_ldexpf(acc[i][j][e], -(G_SCALE + ew));
             }
     }
 }
@@ -487,7 +538,7 @@ __global__ __launch_bounds__(256) void few_dx_sum_kernel(const float* __restrict
 // -------------------------------------------------------------------------------------------- dW
 
 struct FewDw {
-    const __bf16 *x_cols, *g_cols;
+    const _Float16 *x_cols, *g_cols;
     const unsigned* words;
     int hidden, vocab, blocks_v;
     float scale;
@@ -500,17 +551,18 @@ template <int STEPS_T, bool VEC>
 __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
     if (p.words[WORD_COUNT] == 0) return;
     constexpr int HB = STEPS_T == 1 ? 8 : 4;
-    typedef Stream<3 * STEPS_T * HB, 4, 2> S;
-    __shared__ __attribute__((aligned(16))) __bf16 lds[2 * S::STEP];
+    typedef Stream<2 * STEPS_T * HB, 4, 2> S;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * S::STEP];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, vb = blockIdx.x * (int)(blockDim.x >> 6) + wave;
     const int v = 16 * vb + (lane & 15), chunks = (p.hidden + 16 * HB - 1) / (16 * HB);
     const bool live = v < p.vocab;
-    bf16x8 g[STEPS_T][3];
+    const int e = -(G_SCALE + pair_scale_exp(p.words[WORD_WX]));
+    f16x8 g[STEPS_T][2];
 #pragma unroll
     for (int s = 0; s < STEPS_T; ++s)
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
-            g[s][q] = fragment(p.g_cols + (((size_t)min(vb, p.blocks_v - 1) * STEPS_T + s) * 3 + q) * FRAG, lane);
+        for (int q = 0; q < 2; ++q)
+            g[s][q] = fragment(p.g_cols + (((size_t)min(vb, p.blocks_v - 1) * STEPS_T + s) * 2 + q) * FRAG, lane);
     float* row = p.dW + (size_t)min(v, p.vocab - 1) * p.hidden;
     const S x(p.x_cols, lds, wave, lane, chunks);
     auto fetch = [&](int chunk, int k) {
@@ -539,18 +591,19 @@ __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
 #pragma unroll
             for (int k = 0; k < HB; ++k) next[k] = fetch(c + 1, k);
         }
-        const __bf16* xs = lds + (c & 1) * S::STEP;
+        const _Float16* xs = lds + (c & 1) * S::STEP;
 #pragma unroll
         for (int k = 0; k < HB; ++k) {
             f32x4 sum = {};
 #pragma unroll
             for (int s = 0; s < STEPS_T; ++s) {
-                bf16x8 a[3];
+                f16x8 a[2];
 #pragma unroll
-                for (int q = 0; q < 3; ++q) a[q] = fragment(xs + ((k * STEPS_T + s) * 3 + q) * FRAG, lane);
-                mma<3>(a, g[s], sum);
+                for (int q = 0; q < 2; ++q) a[q] = fragment(xs + ((k * STEPS_T + s) * 2 + q) * FRAG, lane);
+                mma<2>(a, g[s], sum);
             }
-            now[k] += sum * p.scale;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) now[k][r] += __builtin_amdgcn_ldexpf(sum[r], e) * p.scale;
             const int h = 16 * (c * HB + k) + 4 * (lane >> 4);
             if (!live) continue;
             if constexpr (VEC) {
@@ -591,6 +644,14 @@ template <class F> void with_blocks(int nb, F&& f) {
     else if (nb == 5) f(std::integral_constant<int, 5>());
     else if (nb == 6) f(std::integral_constant<int, 6>());
     else f(std::integral_constant<int, 8>());
+}
+
+void launch_prepare(laya_ctx* ctx, const Prepare& p, int steps) {
+    if (p.hidden % 4 == 0 && ((uintptr_t)p.x & 15u) == 0)
+        LAYA_LAUNCH(few_prepare_kernel<true>, dim3(steps), dim3(1024), 0, ctx->stream, p);
+    else
+        LAYA_LAUNCH(few_prepare_kernel<false>, dim3(steps), dim3(1024), 0, ctx->stream, p);
+    check_launch("few_prepare_kernel");
 }
 
 template <bool GRAD>
@@ -656,22 +717,24 @@ void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* ls
     const int tiles = (blocks_v + waves - 1) / waves;
     unsigned* words;
     int* row_of;
-    __bf16* x_rows;
+    _Float16* x_rows;
+    int* exps;
     float2* part;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
         ws.take(words, WORDS);
         ws.take(row_of, a.rows);
-        ws.take(x_rows, (size_t)steps * nb * 3 * FRAG);
+        ws.take(exps, 16 * nb);
+        ws.take(x_rows, (size_t)steps * nb * BLOCK);
         ws.take(part, (size_t)tiles * pitch);
     });
-    const Prepare prep{a.x, a.row_weights, a.targets, a.rows, a.hidden, a.vocab, nb, x_rows, nullptr,
+    const Prepare prep{a.x, a.row_weights, a.targets, a.rows, a.hidden, a.vocab, nb, x_rows, nullptr, exps,
                        row_of, nullptr, bad_count, words, row_loss, lse};
-    LAYA_LAUNCH(few_prepare_kernel, dim3(steps), dim3(256), 0, ctx->stream, prep);
-    check_launch("few_prepare_kernel");
+    launch_prepare(ctx, prep, steps);
     FewLogits p{};
     p.W = a.W16 ? (const void*)a.W16 : (const void*)a.W;
     p.bias = a.bias;
     p.x_rows = x_rows;
+    p.exps = exps;
     p.words = words;
     p.hidden = a.hidden;
     p.vocab = a.vocab;
@@ -692,26 +755,28 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
     const int slices = (steps_v + per - 1) / per;
     unsigned* words;
     int *row_of, *place;
-    __bf16 *x_rows, *x_cols, *g_rows, *g_cols;
+    _Float16 *x_rows, *x_cols, *g_rows, *g_cols;
+    int* exps;
     float* part;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
         ws.take(words, WORDS);
         ws.take(row_of, a.rows);
         ws.take(place, a.rows);
-        ws.take(x_rows, (size_t)steps * nb * 3 * FRAG);
-        ws.take(x_cols, (size_t)(2 * steps + 6) * steps_t * 3 * FRAG);  // few_dw reads whole chunks of up to 8 blocks
-        ws.take(g_rows, (size_t)steps_v * nb * 3 * FRAG);
-        ws.take(g_cols, (size_t)blocks_v * steps_t * 3 * FRAG);
+        ws.take(exps, 16 * nb);
+        ws.take(x_rows, (size_t)steps * nb * BLOCK);
+        ws.take(x_cols, (size_t)(2 * steps + 6) * steps_t * BLOCK);  // few_dw reads whole chunks of up to 8 blocks
+        ws.take(g_rows, (size_t)steps_v * nb * BLOCK);
+        ws.take(g_cols, (size_t)blocks_v * steps_t * BLOCK);
         ws.take(part, (size_t)slices * 16 * nb * a.hidden);
     });
-    const Prepare prep{a.x, a.row_weights, a.targets, a.rows, a.hidden, a.vocab, nb, x_rows, x_cols,
+    const Prepare prep{a.x, a.row_weights, a.targets, a.rows, a.hidden, a.vocab, nb, x_rows, x_cols, exps,
                        row_of, place, nullptr, words, nullptr, nullptr};
-    LAYA_LAUNCH(few_prepare_kernel, dim3(steps), dim3(256), 0, ctx->stream, prep);
-    check_launch("few_prepare_kernel");
+    launch_prepare(ctx, prep, steps);
     FewLogits p{};
     p.W = a.W16 ? (const void*)a.W16 : (const void*)a.W;
     p.bias = a.bias;
     p.x_rows = x_rows;
+    p.exps = exps;
     p.words = words;
     p.hidden = a.hidden;
     p.vocab = a.vocab;
@@ -727,7 +792,7 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
     p.scale = a.scale;
     launch_logits<true>(ctx, a, p, nb, waves);
     if (dx) {
-        const FewDx q{p.W, g_rows, a.hidden, a.vocab, steps_v, per, part};
+        const FewDx q{p.W, g_rows, words, a.hidden, a.vocab, steps_v, per, part};
         launch_dx(ctx, a, q, slices, nb);
         LAYA_LAUNCH(few_dx_sum_kernel, dim3((a.hidden + 255) / 256, a.rows), dim3(256), 0, ctx->stream, part, slices,
                     16 * nb, place, a.row_weights, a.scale, a.hidden, dx);
