@@ -704,7 +704,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
         if (bad_count) fill(ctx, reinterpret_cast<float*>(bad_count), 0.0f, 1);
         return;
     }
-    if (a.rows <= VOCAB_FEW) return vocab_few_fwd(ctx, a, row_loss, lse, loss, bad_count);
+    if (vocab_few_rows(a)) return vocab_few_fwd(ctx, a, row_loss, lse, loss, bad_count);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
     const int piece = piece_rows(a.vocab, (size_t)steps_of(a.hidden) * 32 * 2 * planes);
     const int tiles = (a.vocab + TILE - 1) / TILE;
@@ -744,7 +744,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
 
 void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {
     if (a.rows == 0) return;
-    if (a.rows <= VOCAB_FEW) return vocab_few_bwd(ctx, a, lse, dx, dW, db);
+    if (vocab_few_rows(a)) return vocab_few_bwd(ctx, a, lse, dx, dW, db);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = steps_of(a.hidden);
     const int steps_t = steps_of(a.rows);
     const int piece =

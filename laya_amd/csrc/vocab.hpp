@@ -6,7 +6,7 @@
 namespace laya {
 
 constexpr float LOG2E = 1.44269504088896341f;
-constexpr int VOCAB_FEW = 128;  // rows at which the few-row kernels end
+constexpr int VOCAB_FEW = 256;  // rows that the few-row kernels take at most
 
 // Words of a call: labelled rows, targets outside the vocabulary, bits of max|w_t·x_t| and of max|W|, the ways that dx's
 // sum is split, workgroups that have ended.
@@ -45,6 +45,7 @@ __device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v
 // The tiles' statistics part[tile][pitch] into row_loss, lse and the weighted total.
 void vocab_merge(laya_ctx* ctx, const VocabArgs& a, const float2* part, int pitch, int tiles, unsigned* words,
                  const int* row_of, float* row_loss, float* lse, float* loss);
+bool vocab_few_rows(const VocabArgs& a);
 void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count);
 void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db);
 

@@ -1,4 +1,4 @@
-// The vocabulary cross entropy of up to 128 rows, where the table's own bytes are the cost: every kernel reads W (or
+// The vocabulary cross entropy of up to 256 rows, where the table's own bytes are the cost: every kernel reads W (or
 // moves dW) once, straight from memory, and splits it in registers.
 //
 // The products are two-piece fp16 products (split.hpp) as the large ones, three matrix products each, but W is split as it
@@ -41,22 +41,30 @@ __device__ __forceinline__ f16x8 fragment(const _Float16* at, int lane) {
     return *reinterpret_cast<const f16x8*>(at + lane * 8);
 }
 
-// The labelled rows in order, by every workgroup for itself: row_of[j] (LDS) and their number. VOCAB_FEW ≤ 128 rows.
+// The labelled rows in order, by every workgroup for itself: row_of[j] (LDS) and their number. VOCAB_FEW rows at most.
 __device__ __forceinline__ int list_rows(const int* targets, int rows, int vocab, int* row_of, int& bad) {
-    __shared__ int wave_count[2], wave_bad[2];
+    constexpr int WAVES = VOCAB_FEW / 64;
+    __shared__ int wave_count[WAVES], wave_bad[WAVES];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int y = tid < rows ? targets[tid] : LAYA_NO_LABEL;
     const bool has = y >= 0 && y < vocab;
     const unsigned long long m = __ballot(has), wrong = __ballot(!has && y != LAYA_NO_LABEL);
-    if (lane == 0 && wave < 2) {
+    if (lane == 0 && wave < WAVES) {
         wave_count[wave] = __popcll(m);
         wave_bad[wave] = __popcll(wrong);
     }
     __syncthreads();
-    bad = wave_bad[0] + wave_bad[1];
-    if (has) row_of[(wave ? wave_count[0] : 0) + __popcll(m & ((1ull << lane) - 1))] = tid;
+    int before = 0, count = 0;
+    bad = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += wave_count[w];
+        count += wave_count[w];
+        bad += wave_bad[w];
+    }
+    if (has) row_of[before + __popcll(m & ((1ull << lane) - 1))] = tid;
     __syncthreads();
-    return wave_count[0] + wave_count[1];
+    return count;
 }
 
 struct Prepare {
@@ -81,8 +89,8 @@ __global__ __launch_bounds__(1024) void few_prepare_kernel(Prepare p) {
     int bad;
     if (tid == 0) whole = 0;
     const int count = list_rows(p.targets, p.rows, p.vocab, row_of, bad);
-    {  // thread t four columns of row t / 8 of this step
-        const int j = tid >> 3, c = 32 * step + 4 * (tid & 7);
+    for (int j = tid >> 3; j < 16 * p.blocks_t; j += 128) {  // thread t four columns of row t / 8 of this step
+        const int c = 32 * step + 4 * (tid & 7);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             tile[j][4 * (tid & 7) + i] =
@@ -131,18 +139,17 @@ __global__ __launch_bounds__(1024) void few_prepare_kernel(Prepare p) {
     const int o = tid & 3, steps_t = (p.blocks_t + 1) / 2;
     float v[8];
     f16x8 f[2];
-    if (tid < 512) {  // row r over h, octet o
-        const int r = tid >> 2, tb = r >> 4;
-        if (tb >= p.blocks_t) return;
+    for (int r = tid >> 2; r < 16 * p.blocks_t; r += 256) {  // row r over h, octet o
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[r][8 * o + i];
         split8(v, exp2_int(row_exp[r]), f);
-        _Float16* to = p.x_rows + ((size_t)step * p.blocks_t + tb) * BLOCK + (o * 16 + (r & 15)) * 8;
+        _Float16* to = p.x_rows + ((size_t)step * p.blocks_t + (r >> 4)) * BLOCK + (o * 16 + (r & 15)) * 8;
 #pragma unroll
         for (int k = 0; k < 2; ++k) *reinterpret_cast<f16x8*>(to + k * FRAG) = f[k];
-    } else if (p.x_cols) {  // column 32·step + r over t, octet o of step s
-        const int r = ((tid - 512) >> 2) & 31, s = (tid - 512) >> 7;
-        if (s >= steps_t) return;
+    }
+    if (!p.x_cols) return;
+    for (int s = tid >> 7; s < steps_t; s += 8) {  // column 32·step + r over t, octet o of step s
+        const int r = (tid >> 2) & 31;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int t = 32 * s + 8 * o + i;
@@ -222,7 +229,6 @@ struct FewLogits {
     float scale;
 };
 
-constexpr int RING = 4;
 
 // load8 as two loads (fp32) or one (bf16) whatever the column (aligned rows of a multiple of 8); the caller clears what lies
 // behind K.
@@ -241,31 +247,45 @@ __device__ __forceinline__ void load8_always(const __bf16* row, int c, int K, fl
     for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
 }
 
+// Blocks of 16 rows of W a wave takes: with many rows of x it is their reads from LDS that two blocks share.
+constexpr int wave_blocks(int nb) { return nb >= 8 ? 2 : 1; }
+// Steps of a ring: what is under way of W waits in registers.
+constexpr int ring_of(int nb) { return nb >= 12 ? 3 : 4; }
+
 // A workgroup is as many waves, WAVES at least, as spread the table's blocks of 16 rows evenly over the CUs.
 template <int NB, typename TW, bool VEC, bool GRAD, int WAVES>
-__global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = sizeof(TW) == 2 ? 1 : 2;
+__global__ __launch_bounds__(1024 / wave_blocks(NB), 1) void few_logits_kernel(FewLogits p) {
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, VB = wave_blocks(NB), RING = ring_of(NB);
+    constexpr int LOADS = VB * (sizeof(TW) == 2 ? 1 : 2);
     typedef Stream<2 * NB, WAVES, RING> S;
     constexpr int PITCH = 36, ROOM = GRAD ? 16 * 16 * PITCH * 2 : 16 * 16 * NB * 4;  // what the end needs
     __shared__ __attribute__((aligned(16))) _Float16 lds[RING * S::STEP < ROOM ? ROOM : RING * S::STEP];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, waves = blockDim.x >> 6, steps = p.steps;
-    const int v0 = (blockIdx.x * waves + wave) * 16;
-    const TW* row = static_cast<const TW*>(p.W) + (size_t)min(v0 + (lane & 15), p.vocab - 1) * p.hidden;
+    const int v0 = (blockIdx.x * waves + wave) * (16 * VB);
+    const TW* row[VB];
+#pragma unroll
+    for (int i = 0; i < VB; ++i)
+        row[i] = static_cast<const TW*>(p.W) + (size_t)min(v0 + 16 * i + (lane & 15), p.vocab - 1) * p.hidden;
     const S x(p.x_rows, lds, wave, lane, steps);
-    auto load = [&](int s, float (&w)[8]) {
+    auto load = [&](int s, float (&w)[VB][8]) {
         const int c = 32 * s + 8 * (lane >> 4);
-        if constexpr (VEC)
-            load8_always(row, c, p.hidden, w);
-        else
-            load8<false>(row, c, p.hidden, w);
+#pragma unroll
+        for (int i = 0; i < VB; ++i) {
+            if constexpr (VEC)
+                load8_always(row[i], c, p.hidden, w[i]);
+            else
+                load8<false>(row[i], c, p.hidden, w[i]);
+        }
     };
-    float w[RING][8];
+    float w[RING][VB][8];
     int e = 126;           // of the wave's scale
     float limit = 0.0f;    // magnitudes from here on need another
     float top = 0.0f;      // the lane's largest
-    f32x4 acc[NB];
+    f32x4 acc[VB][NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[j] = f32x4{};
+    for (int i = 0; i < VB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{};
 #pragma unroll
     for (int k = 0; k < RING - 1; ++k) {
         x.start(k);
@@ -283,65 +303,88 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
         __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
         if (VEC && 32 * s + 8 * (lane >> 4) >= p.hidden)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[K][e] = 0.0f;
+            for (int i = 0; i < VB; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[K][i][k] = 0.0f;
         float m = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(w[K][k]));
+        for (int i = 0; i < VB; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(w[K][i][k]));
         if (__any(m >= limit)) {  // a new scale (of infinities, none: they reach the sums as such)
             unsigned bits = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) bits = max(bits, amax_bits(w[K][k]));
+            for (int i = 0; i < VB; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) bits = max(bits, amax_bits(w[K][i][k]));
             m = __builtin_bit_cast(float, bits);
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o, 64));
             const int to = min(e, pair_scale_exp(bits) - 3);
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int i = 0; i < VB; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], to - e);
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_ldexpf(acc[i][j][r], to - e);
             e = to;
             limit = exp2_int(min(15 - e, 127));
         }
         if (GRAD) top = fmaxf(top, m);
-        f16x8 a[2];
-        split8(w[K], exp2_int(max(e, -126)), a);
+        f16x8 a[VB][2];
+#pragma unroll
+        for (int i = 0; i < VB; ++i) split8(w[K][i], exp2_int(max(e, -126)), a[i]);
         const _Float16* xs = lds + K * S::STEP;
+        // A block of x ahead, and no more (the scheduler would hold them all).
+        f16x8 b[2][2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) b[0][q] = fragment(xs + q * FRAG, lane);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            f16x8 b[2];
+            if (j + 1 < NB)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) b[q] = fragment(xs + (2 * j + q) * FRAG, lane);
-            mma<PW>(a, b, acc[j]);
+                for (int q = 0; q < 2; ++q) b[(j + 1) & 1][q] = fragment(xs + (2 * (j + 1) + q) * FRAG, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < VB; ++i) mma<PW>(a[i], b[j & 1], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    for (int s = 0; s < steps; s += 4) {
+    for (int s = 0; s < steps; s += RING) {
         step(s, std::integral_constant<int, 0>());
         if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
         if (s + 2 < steps) step(s + 2, std::integral_constant<int, 2>());
-        if (s + 3 < steps) step(s + 3, std::integral_constant<int, 3>());
+        if constexpr (RING == 4)
+            if (s + 3 < steps) step(s + 3, std::integral_constant<int, 3>());
     }
     packed::wait_copies<0>();
     const int count = (int)p.words[WORD_COUNT];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int v = v0 + 4 * (lane >> 4) + r;
-        const float b = v < p.vocab ? (p.bias ? p.bias[v] : 0.0f) : -__builtin_inff();
+    for (int i = 0; i < VB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-            acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], -(e + p.exps[16 * j + (lane & 15)])) + b;
-    }
+        for (int r = 0; r < 4; ++r) {
+            const int v = v0 + 16 * i + 4 * (lane >> 4) + r;
+            const float b = v < p.vocab ? (p.bias ? p.bias[v] : 0.0f) : -__builtin_inff();
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                acc[i][j][r] = __builtin_amdgcn_ldexpf(acc[i][j][r], -(e + p.exps[16 * j + (lane & 15)])) + b;
+        }
     if constexpr (!GRAD) {
         float2* red = reinterpret_cast<float2*>(lds);  // [wave][16·NB]
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             float m = -__builtin_inff(), s = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[j][r]);
+            for (int i = 0; i < VB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const float at = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[j][r] - at) * LOG2E);
+            for (int i = 0; i < VB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * LOG2E);
             s += __shfl_xor(s, 16, 64);
             s += __shfl_xor(s, 32, 64);
             if (lane < 16) red[wave * (16 * NB) + 16 * j + lane] = make_float2(m, s);
@@ -367,56 +410,60 @@ __global__ __launch_bounds__(1024, 1) void few_logits_kernel(FewLogits p) {
         if (v0 >= p.blocks_v * 16) return;
         constexpr int STEPS_T = (NB + 1) / 2;
         float* turn = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
-        f32x4 db = {};
 #pragma unroll
-        for (int ts = 0; ts < STEPS_T; ++ts) {
+        for (int i = 0; i < VB; ++i) {
+            const int vb = v0 + 16 * i;
+            f32x4 db = {};
 #pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-                const int j = 2 * ts + jj, t = 16 * j + (lane & 15);
-                f32x4 g = {};
-                if (j < NB) {
-                    const bool live = t < count;
-                    const int r = live ? p.row_of[t] : 0;
-                    const float lse = live ? p.lse[r] : 0.0f;
-                    const int y = (live ? p.targets[r] : -1) - (v0 + 4 * (lane >> 4));
+            for (int ts = 0; ts < STEPS_T; ++ts) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float q = __builtin_amdgcn_exp2f((acc[j][e] - lse) * LOG2E);
-                        q -= y == e ? 1.0f : 0.0f;
-                        g[e] = live ? q * (float)(1 << G_SCALE) : 0.0f;
+                for (int jj = 0; jj < 2; ++jj) {
+                    const int j = 2 * ts + jj, t = 16 * j + (lane & 15);
+                    f32x4 g = {};
+                    if (j < NB) {
+                        const bool live = t < count;
+                        const int r = live ? p.row_of[t] : 0;
+                        const float lse = live ? p.lse[r] : 0.0f;
+                        const int y = (live ? p.targets[r] : -1) - (vb + 4 * (lane >> 4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float q = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * LOG2E);
+                            q -= y == e ? 1.0f : 0.0f;
+                            g[e] = live ? q * (float)(1 << G_SCALE) : 0.0f;
+                        }
+                        const float wt = live ? (p.weights ? p.weights[r] : 1.0f) : 0.0f;
+                        db += live ? g * wt : f32x4{};
+                        f16x4 f[2];
+                        split2h_4(g, 1.0f, f[0], f[1]);
+                        _Float16* to = p.g_rows + ((size_t)(vb >> 5) * NB + j) * BLOCK +
+                                     ((((vb >> 4) & 1) * 2 + (lane >> 5)) * 16 + (lane & 15)) * 8 + 4 * ((lane >> 4) & 1);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) *reinterpret_cast<f16x4*>(to + q * FRAG) = f[q];
                     }
-                    const float wt = live ? (p.weights ? p.weights[r] : 1.0f) : 0.0f;
-                    db += live ? g * wt : f32x4{};
-                    f16x4 f[2];
-                    split2h_4(g, 1.0f, f[0], f[1]);
-                    _Float16* to = p.g_rows + ((size_t)(v0 >> 5) * NB + j) * BLOCK +
-                                 ((((v0 >> 4) & 1) * 2 + (lane >> 5)) * 16 + (lane & 15)) * 8 + 4 * ((lane >> 4) & 1);
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) *reinterpret_cast<f16x4*>(to + q * FRAG) = f[q];
+                    for (int e = 0; e < 4; ++e) turn[(4 * (lane >> 4) + e) * PITCH + 16 * jj + (lane & 15)] = g[e];
                 }
+                float v[8];
+                f16x8 f[2];
+                const float* at = turn + (lane & 15) * PITCH + 8 * (lane >> 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) turn[(4 * (lane >> 4) + e) * PITCH + 16 * jj + (lane & 15)] = g[e];
+                for (int e = 0; e < 8; ++e) v[e] = at[e];
+                split8(v, 1.0f, f);
+                _Float16* to = p.g_cols + ((size_t)(vb >> 4) * STEPS_T + ts) * BLOCK + lane * 8;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) *reinterpret_cast<f16x8*>(to + q * FRAG) = f[q];
             }
-            float v[8];
-            f16x8 f[2];
-            const float* at = turn + (lane & 15) * PITCH + 8 * (lane >> 4);
+            if (p.db) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = at[e];
-            split8(v, 1.0f, f);
-            _Float16* to = p.g_cols + ((size_t)(v0 >> 4) * STEPS_T + ts) * BLOCK + lane * 8;
+                for (int o = 1; o < 16; o <<= 1)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) *reinterpret_cast<f16x8*>(to + q * FRAG) = f[q];
-        }
-        if (p.db) {
+                    for (int e = 0; e < 4; ++e) db[e] += __shfl_xor(db[e], o, 64);
+                const int v = vb + 4 * (lane >> 4);
+                if ((lane & 15) == 0)
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) db[e] += __shfl_xor(db[e], o, 64);
-            const int v = v0 + 4 * (lane >> 4);
-            if ((lane & 15) == 0)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (v + e < p.vocab) p.db[v + e] += db[e] * (1.0f / (1 << G_SCALE)) * p.scale;
+                    for (int e = 0; e < 4; ++e)
+                        if (v + e < p.vocab) p.db[v + e] += db[e] * (1.0f / (1 << G_SCALE)) * p.scale;
+            }
         }
     }
 }
@@ -435,7 +482,7 @@ struct FewDx {
 // lane's two blocks come with one load a row (PAIR: rows of pairs).
 template <int NB, typename TW, bool PAIR>
 __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = PAIR ? 8 : 16;
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = PAIR ? 8 : 16, RING = 4;
     typedef Stream<2 * NB, 8, RING> S;
     __shared__ __attribute__((aligned(16))) _Float16 lds[RING * S::STEP];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -482,24 +529,29 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
         g.start(s + RING - 1);
         load(s + RING - 1, w[(K + RING - 1) % RING]);
         __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
-        f16x8 a[2][2];
+        f16x8 a[2][2], b[2][2];
         split8(w[K][0], sc, a[0]);
         split8(w[K][1], sc, a[1]);
         const _Float16* gs = lds + K * S::STEP;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            f16x8 b[2];
+        for (int q = 0; q < 2; ++q) b[0][q] = fragment(gs + q * FRAG, lane);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) b[q] = fragment(gs + (2 * j + q) * FRAG, lane);
-            mma<PW>(a[0], b, acc[0][j]);
-            mma<PW>(a[1], b, acc[1][j]);
+        for (int j = 0; j < NB; ++j) {
+            if (j + 1 < NB)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) b[(j + 1) & 1][q] = fragment(gs + (2 * (j + 1) + q) * FRAG, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            mma<PW>(a[0], b[j & 1], acc[0][j]);
+            mma<PW>(a[1], b[j & 1], acc[1][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    for (int s = 0; s < steps; s += 4) {
+    for (int s = 0; s < steps; s += RING) {
         step(s, std::integral_constant<int, 0>());
         if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
         if (s + 2 < steps) step(s + 2, std::integral_constant<int, 2>());
-        if (s + 3 < steps) step(s + 3, std::integral_constant<int, 3>());
+        if constexpr (RING == 4)
+            if (s + 3 < steps) step(s + 3, std::integral_constant<int, 3>());
     }
     packed::wait_copies<0>();
 #pragma unroll
@@ -550,7 +602,7 @@ struct FewDw {
 template <int STEPS_T, bool VEC>
 __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
     if (p.words[WORD_COUNT] == 0) return;
-    constexpr int HB = STEPS_T == 1 ? 8 : 4;
+    constexpr int HB = STEPS_T == 1 ? 8 : STEPS_T <= 4 ? 4 : 2;
     typedef Stream<2 * STEPS_T * HB, 4, 2> S;
     __shared__ __attribute__((aligned(16))) _Float16 lds[2 * S::STEP];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, vb = blockIdx.x * (int)(blockDim.x >> 6) + wave;
@@ -625,14 +677,16 @@ bool aligned_table(const VocabArgs& a) {
 }
 int blocks_of(const VocabArgs& a) {
     const int b = (a.rows + 15) / 16;
-    return !aligned_table(a) || b == 7 ? 8 : b;
+    if (!aligned_table(a)) return 8;
+    return b <= 6 ? b : b <= 8 ? 8 : b <= 10 ? 10 : b <= 12 ? 12 : 16;
 }
 
-// Waves of a workgroup of few_logits and few_dw, a block of 16 rows of W each: as few as take the table in the rounds that
-// 16 would take, one workgroup a CU, and 4 at least.
-int waves_of(const laya_ctx* ctx, int blocks_v) {
+// Waves of a workgroup that takes `each` blocks of 16 rows of W a wave: as few as take the table in the rounds that 16
+// blocks a workgroup would take, one workgroup a CU, and 4 at least.
+int waves_of(const laya_ctx* ctx, int blocks_v, int each = 1) {
     const int rounds = (blocks_v + 16 * ctx->cu_count - 1) / (16 * ctx->cu_count);
-    return std::max(4, (blocks_v + rounds * ctx->cu_count - 1) / (rounds * ctx->cu_count));
+    const int units = (blocks_v + each - 1) / each;
+    return std::max(4, (units + rounds * ctx->cu_count - 1) / (rounds * ctx->cu_count));
 }
 
 // f(the number of blocks as a constant).
@@ -643,7 +697,10 @@ template <class F> void with_blocks(int nb, F&& f) {
     else if (nb == 4) f(std::integral_constant<int, 4>());
     else if (nb == 5) f(std::integral_constant<int, 5>());
     else if (nb == 6) f(std::integral_constant<int, 6>());
-    else f(std::integral_constant<int, 8>());
+    else if (nb == 8) f(std::integral_constant<int, 8>());
+    else if (nb == 10) f(std::integral_constant<int, 10>());
+    else if (nb == 12) f(std::integral_constant<int, 12>());
+    else f(std::integral_constant<int, 16>());
 }
 
 void launch_prepare(laya_ctx* ctx, const Prepare& p, int steps) {
@@ -655,8 +712,9 @@ void launch_prepare(laya_ctx* ctx, const Prepare& p, int steps) {
 }
 
 template <bool GRAD>
-void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p, int nb, int waves) {
-    const dim3 grid((p.blocks_v + waves - 1) / waves), block(64 * waves);
+void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p, int nb) {
+    const int each = wave_blocks(nb), waves = waves_of(ctx, p.blocks_v, each);
+    const dim3 grid((p.blocks_v + waves * each - 1) / (waves * each)), block(64 * waves);
     ProfileScope scope(ctx, "vocab_few_logits", 2.0 * a.rows * a.hidden * a.vocab,
                        (a.W16 ? 2.0 : 4.0) * a.hidden * a.vocab);
     if (!aligned_table(a)) {
@@ -667,12 +725,13 @@ void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p, int nb
     } else {
         with_blocks(nb, [&](auto n) {
             constexpr int NB = decltype(n)::value;
-            if (a.W16 && waves >= 8)
-                LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, 8>), grid, block, 0, ctx->stream, p);
+            constexpr int MANY = wave_blocks(NB) == 2 ? 6 : 8;
+            if (a.W16 && waves >= MANY)
+                LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, MANY>), grid, block, 0, ctx->stream, p);
             else if (a.W16)
                 LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, 4>), grid, block, 0, ctx->stream, p);
-            else if (waves >= 8)
-                LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, 8>), grid, block, 0, ctx->stream, p);
+            else if (waves >= MANY)
+                LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, MANY>), grid, block, 0, ctx->stream, p);
             else
                 LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, 4>), grid, block, 0, ctx->stream, p);
         });
@@ -711,10 +770,12 @@ void launch_dw(laya_ctx* ctx, const VocabArgs& a, const FewDw& p, int waves) {
 
 }  // namespace
 
+bool vocab_few_rows(const VocabArgs& a) { return a.rows <= (aligned_table(a) ? VOCAB_FEW : 128); }
+
 void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count) {
     const int nb = blocks_of(a), pitch = 16 * nb, steps = packed::steps_of(a.hidden);
-    const int blocks_v = 2 * packed::steps_of(a.vocab), waves = waves_of(ctx, blocks_v);
-    const int tiles = (blocks_v + waves - 1) / waves;
+    const int blocks_v = 2 * packed::steps_of(a.vocab), rows_of_wg = wave_blocks(nb) * waves_of(ctx, blocks_v, wave_blocks(nb));
+    const int tiles = (blocks_v + rows_of_wg - 1) / rows_of_wg;
     unsigned* words;
     int* row_of;
     _Float16* x_rows;
@@ -742,7 +803,7 @@ void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* ls
     p.blocks_v = blocks_v;
     p.part = part;
     p.pitch = pitch;
-    launch_logits<false>(ctx, a, p, nb, waves);
+    launch_logits<false>(ctx, a, p, nb);
     vocab_merge(ctx, a, part, pitch, tiles, words, row_of, row_loss, lse, loss);
 }
 
@@ -790,7 +851,7 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
     p.g_cols = g_cols;
     p.db = db;
     p.scale = a.scale;
-    launch_logits<true>(ctx, a, p, nb, waves);
+    launch_logits<true>(ctx, a, p, nb);
     if (dx) {
         const FewDx q{p.W, g_rows, words, a.hidden, a.vocab, steps_v, per, part};
         launch_dx(ctx, a, q, slices, nb);
@@ -803,7 +864,10 @@ void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* d
         if (steps_t == 1) launch_dw<1>(ctx, a, q, waves);
         else if (steps_t == 2) launch_dw<2>(ctx, a, q, waves);
         else if (steps_t == 3) launch_dw<3>(ctx, a, q, waves);
-        else launch_dw<4>(ctx, a, q, waves);
+        else if (steps_t == 4) launch_dw<4>(ctx, a, q, waves);
+        else if (steps_t == 5) launch_dw<5>(ctx, a, q, waves);
+        else if (steps_t == 6) launch_dw<6>(ctx, a, q, waves);
+        else launch_dw<8>(ctx, a, q, waves);
     }
 }
 
