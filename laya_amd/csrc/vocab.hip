@@ -675,9 +675,15 @@ void pack_states(laya_ctx* ctx, const VocabArgs& a, const int* row_of, unsigned*
     launch_pack<float, 2>(ctx, p, groups_of(a.rows));
 }
 
-// Rows of the vocabulary a piece takes: whole tiles, pieces of about equal size, `each` bytes a row.
-int piece_rows(int vocab, size_t each) {
-    const long most = std::max<long>(TILE, (long)(PIECE_BYTES / each) / TILE * TILE);
+// Rows of the vocabulary a piece takes: whole tiles, pieces of about equal size, `each` bytes a row. Under a memory cap no
+// more than fits what the cap leaves beside the `fixed` bytes of the workspace.
+int piece_rows(const laya_ctx* ctx, int vocab, size_t each, size_t fixed) {
+    size_t bytes = PIECE_BYTES;
+    if (ctx->cap) {
+        const size_t taken = ctx->in_use - ctx->scratch[VOCAB_SLOT].bytes + fixed + (64 << 10);
+        bytes = std::min(bytes, ctx->cap > taken ? ctx->cap - taken : 0);
+    }
+    const long most = std::max<long>(TILE, (long)(bytes / each) / TILE * TILE);
     const long pieces = (vocab + most - 1) / most;
     return (int)std::min<long>(pad_tile((vocab + pieces - 1) / pieces), pad_tile(vocab));
 }
@@ -706,8 +712,9 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
     }
     if (vocab_few_rows(a)) return vocab_few_fwd(ctx, a, row_loss, lse, loss, bad_count);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
-    const int piece = piece_rows(a.vocab, (size_t)steps_of(a.hidden) * 32 * 2 * planes);
     const int tiles = (a.vocab + TILE - 1) / TILE;
+    const int piece = piece_rows(ctx, a.vocab, (size_t)steps_of(a.hidden) * 64 * planes + 8,
+                                 2 * halves(a.rows, a.hidden, 2) + 8 * ((size_t)tiles + 1) * pitch);
     unsigned* words;
     int *row_of, *ex, *ew;
     float* padded;
@@ -747,10 +754,12 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
     if (vocab_few_rows(a)) return vocab_few_bwd(ctx, a, lse, dx, dW, db);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows), steps_h = steps_of(a.hidden);
     const int steps_t = steps_of(a.rows);
-    const int piece =
-        piece_rows(a.vocab, (size_t)steps_h * 32 * 2 * planes + (size_t)steps_t * 32 * 4);
-    const int cap_rows = std::max(pitch, std::min(MAX_SPLITS * pitch, 32768));
+    // dx's partial sums: as many rows as its splits may come to; under a memory cap a few.
+    const int cap_rows = std::max(pitch, std::min((ctx->cap ? 2 : MAX_SPLITS) * pitch, 32768));
     const int tiles_t = pitch / TILE, tiles_h = (a.hidden + TILE - 1) / TILE;
+    const int piece = piece_rows(ctx, a.vocab, (size_t)steps_h * 64 * planes + (size_t)steps_t * 128 + 8 + (db ? 16 * tiles_t : 0),
+                                 4 * halves(a.rows, a.hidden, 2) + 16 * (size_t)pitch +
+                                     (dx ? 4 * (size_t)cap_rows * a.hidden : 0));
     unsigned* words;
     int *row_of, *place, *ex, *ew;
     float *padded, *part, *db_part;
