@@ -34,12 +34,14 @@ struct Shape {
     size_t x0, ab0;           // where the run's first lie
     int chunks, chunk0;       // partial sums of squares a matrix has, and where the run's first lie
     int unit0;                // the launch's units before the run
-    int tiles_m, tiles_n;     // of a matrix (gram, poly: tiles_n x tiles_n, those on and below the diagonal)
+    int tiles, across;        // of a matrix, and of those a row of its tiles has (update)
+    int turn;                 // the XCD that the run's first matrix goes to
 };
 constexpr int MAX_SHAPES = 16;
 
 struct Batch {
     int shapes, units;
+    int together;  // see find_tile
     Shape s[MAX_SHAPES];
 };
 
@@ -157,8 +159,26 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Batch b, Source f, const
     const double inverse = sum > 0.0 ? 1.0 / sqrt(sum) : sum != sum ? sum : 0.0;
     const float cf = f.coef ? *f.coef : 1.0f;
     float v[8] = {};
-    if (row < s.rows) {
-        const size_t from = base + (size_t)row * s.cols;
+    const size_t from = base + (size_t)row * s.cols;
+    const float* one = f.x ? f.x : f.grads;
+    const uintptr_t low = (uintptr_t)(one + from) | (f.x ? 0 : (uintptr_t)(f.momentum + from));
+    if (row < s.rows && c + 8 <= s.cols && (low & 15u) == 0 && s.cols % 4 == 0) {
+        f32x4 a[2], m[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) a[q] = *reinterpret_cast<const f32x4*>(one + from + c + 4 * q);
+        if (!f.x) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                m[q] = *reinterpret_cast<const f32x4*>(f.momentum + from + c + 4 * q);
+                if (f.zero_grads) *reinterpret_cast<f32x4*>(f.grads + from + c + 4 * q) = f32x4{};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = a[i >> 2][i & 3];
+            v[i] = f.x ? x : f.nesterov ? fmaf(f.mu, m[i >> 2][i & 3], x * cf) : m[i >> 2][i & 3];
+        }
+    } else if (row < s.rows) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (c + i < s.cols) {
@@ -209,22 +229,37 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Batch b, Source f, const
 
 // ------------------------------------------------------------------------------------------ products
 
-// Tiles of 256, 128 and 64; how many workgroups share a CU.
-struct T256 {
-    template <bool TA> using Tile = packed::Tile<2, 4, 8, 4, 2, 2, TA, false, 2>;
-    static constexpr int SIZE = 256, PER_CU = 1;
+// Square tiles, how many workgroups share a CU, and the waves of one.
+template <int SIZE_, int WAVES_N, int PER_CU_, int RING>
+struct Config {
+    static constexpr int SIZE = SIZE_, PER_CU = PER_CU_, WN = WAVES_N, BM = SIZE / 32, BN = SIZE / 16 / WAVES_N;
+    template <bool TA> using Tile = packed::Tile<2, WAVES_N, BM, BN, 2, 2, TA, false, RING>;
 };
-struct T128 {
-    template <bool TA> using Tile = packed::Tile<2, 2, 4, 4, 2, 2, TA, false, 2>;
-    static constexpr int SIZE = 128, PER_CU = 2;
-};
-struct T64 {
-    template <bool TA> using Tile = packed::Tile<2, 2, 2, 2, 2, 2, TA, false, 4>;
-    static constexpr int SIZE = 64, PER_CU = 2;
-};
+typedef Config<256, 4, 1, 2> T256;
+typedef Config<128, 2, 2, 2> T128;
+typedef Config<64, 2, 2, 4> T64;
 
-__device__ __forceinline__ int triangle_of(const Shape& s) { return s.tiles_n * (s.tiles_n + 1) / 2; }
-__device__ __forceinline__ int rectangle_of(const Shape& s) { return s.tiles_n * s.tiles_m; }
+// The workgroup's tile. Of a run of `many` matrices the tiles of one run on one XCD (workgroups go round the 8), so that its
+// packed rows come into one L2; runs of few spread over all.
+struct Where {
+    int shape, index, tile;
+};
+__device__ __forceinline__ bool find_tile(const Batch& b, int u, Where& at) {
+    int k = 0;
+    while (k + 1 < b.shapes && u >= b.s[k + 1].unit0) ++k;
+    const Shape& s = b.s[k];
+    const int in = u - s.unit0;
+    at.shape = k;
+    if (b.together) {
+        const int slot = in >> 3;
+        at.index = slot / s.tiles * 8 + ((in + b.s[k].turn) & 7);
+        at.tile = slot % s.tiles;
+    } else {
+        at.index = in / s.tiles;
+        at.tile = in % s.tiles;
+    }
+    return at.index < s.count;
+}
 
 // Row ti and column tj ≤ ti of the u-th tile on or below the diagonal.
 __device__ __forceinline__ void triangle_tile(int u, int& ti, int& tj) {
@@ -239,12 +274,13 @@ __global__ __launch_bounds__(C::template Tile<false>::THREADS, C::PER_CU) void m
     Batch b, const _Float16* __restrict__ in, _Float16* __restrict__ out) {
     typedef typename C::template Tile<false> T;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
-    constexpr int WN = C::SIZE == 256 ? 4 : 2, BM = C::SIZE / 32, BN = C::SIZE / 16 / WN;
+    constexpr int WN = C::WN, BM = C::BM, BN = C::BN;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
-    const Matrix at = find(b, blockIdx.x, triangle_of);
+    Where at;
+    if (!find_tile(b, blockIdx.x, at)) return;
     const Shape& s = b.s[at.shape];
     int ti, tj;
-    triangle_tile(at.unit, ti, tj);
+    triangle_tile(at.tile, ti, tj);
     const int steps = POLY ? s.steps_n : s.steps_m;
     const _Float16* from = in + (POLY ? s.ab0 + at.index * s.ab : s.x0 + at.index * s.x);
     _Float16* to = out + s.ab0 + at.index * s.ab;
@@ -307,11 +343,12 @@ __global__ __launch_bounds__(C::template Tile<true>::THREADS, C::PER_CU) void mu
     Batch b, const _Float16* __restrict__ X, const _Float16* __restrict__ B, _Float16* __restrict__ out, Sink sink) {
     typedef typename C::template Tile<true> T;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
-    constexpr int WN = C::SIZE == 256 ? 4 : 2, BM = C::SIZE / 32, BN = C::SIZE / 16 / WN;
+    constexpr int WN = C::WN, BM = C::BM, BN = C::BN;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / WN, wn = wave % WN;
-    const Matrix at = find(b, blockIdx.x, rectangle_of);
+    Where at;
+    if (!find_tile(b, blockIdx.x, at)) return;
     const Shape& s = b.s[at.shape];
-    const int ti = at.unit / s.tiles_n, tj = at.unit % s.tiles_n;
+    const int ti = at.tile / s.across, tj = at.tile % s.across;
     const Operand x{X + s.x0 + at.index * s.x, s.steps_m, s.groups_n}, bb{B + s.ab0 + at.index * s.ab, s.steps_n, s.groups_n};
     typename T::Acc acc;
     T::product(x, bb, ti * T::MG, tj * T::NG, 0, s.steps_n, lds, acc, wave, lane);
@@ -338,25 +375,41 @@ __global__ __launch_bounds__(C::template Tile<true>::THREADS, C::PER_CU) void mu
         float* to = (sink.out ? sink.out : sink.params) + base;
         const float k = sink.out ? unscale : -sink.rate * sink.multipliers[which] * unscale;
         const bool wide = s.rows <= s.cols, vec = wide && s.cols % 4 == 0 && ((uintptr_t)to & 15u) == 0;
+        // A row block's old values are read together, so that their latencies overlap.
 #pragma unroll
-        for (int i = 0; i < BM; ++i)
+        for (int i = 0; i < BM; ++i) {
+            const int col = i0 + 16 * i + 4 * (lane >> 4), row = j0 + (lane & 15);  // of X; block j: row + 16·j
+            f32x4 old[BN];
+            if (!sink.out) {
+#pragma unroll
+                for (int j = 0; j < BN; ++j) {
+                    const int r = min(row + 16 * j, s.n - 1);
+                    if (vec) {
+                        old[j] = *reinterpret_cast<const f32x4*>(to + (size_t)r * s.cols + min(col, s.m - 4));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int c = min(col + e, s.m - 1);
+                            old[j][e] = to[wide ? (size_t)r * s.cols + c : (size_t)c * s.cols + r];
+                        }
+                    }
+                }
+            }
 #pragma unroll
             for (int j = 0; j < BN; ++j) {
-                const int row = j0 + 16 * j + (lane & 15), col = i0 + 16 * i + 4 * (lane >> 4);  // of X
-                if (row >= s.n || col >= s.m) continue;
+                const int r = row + 16 * j;
                 f32x4 v = acc[i][j] * k;
+                if (!sink.out) v += old[j] * sink.decay;
+                if (r >= s.n) continue;
                 if (vec) {
-                    f32x4* p = reinterpret_cast<f32x4*>(to + (size_t)row * s.cols + col);
-                    *p = sink.out ? v : *p * sink.decay + v;
+                    if (col < s.m) *reinterpret_cast<f32x4*>(to + (size_t)r * s.cols + col) = v;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (col + e < s.m) {
-                            float* p = to + (wide ? (size_t)row * s.cols + col + e : (size_t)(col + e) * s.cols + row);
-                            *p = sink.out ? v[e] : *p * sink.decay + v[e];
-                        }
+                        if (col + e < s.m) to[wide ? (size_t)r * s.cols + col + e : (size_t)(col + e) * s.cols + r] = v[e];
                 }
             }
+        }
     }
 }
 
@@ -364,37 +417,59 @@ __global__ __launch_bounds__(C::template Tile<true>::THREADS, C::PER_CU) void mu
 
 int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-// Sets the units of a launch with tiles of `size`; returns how many there are.
-int tile_units(Batch& b, int size, bool triangle) {
-    int units = 0;
+// Sets the units of a launch with tiles of size x size.
+void tile_units(Batch& b, int size, bool triangle) {
+    int units = 0, before = 0, matrices = 0;
+    for (int k = 0; k < b.shapes; ++k) matrices += b.s[k].count;
+    b.together = matrices >= 32;
     for (int k = 0; k < b.shapes; ++k) {
         Shape& s = b.s[k];
-        s.tiles_n = ceil_div(s.n, size);
-        s.tiles_m = ceil_div(s.m, size);
+        s.across = ceil_div(s.n, size);
+        s.tiles = triangle ? s.across * (s.across + 1) / 2 : ceil_div(s.m, size) * s.across;
         s.unit0 = units;
-        units += s.count * (triangle ? s.tiles_n * (s.tiles_n + 1) / 2 : s.tiles_n * s.tiles_m);
+        s.turn = before & 7;
+        units += (b.together ? (s.count + 7) / 8 * 8 : s.count) * s.tiles;
+        before += s.count;
     }
-    return b.units = units;
+    b.units = units;
 }
 
-// The tile for a launch: the one whose rounds over the chip take least. A step of 32 of K costs a CU about 1.6 us with a
-// 256 x 256 tile, 1.0 us with two of 128 x 128, 0.45 us with two of 64 x 64.
-int pick_tile(laya_ctx* ctx, Batch& b, bool triangle) {
-    const struct { int size, slots; double step; } t[3] = {
-        {256, ctx->cu_count, 1.6}, {128, 2 * ctx->cu_count, 1.0}, {64, 2 * ctx->cu_count, 0.45}};
+// The tile for a launch, by an estimate of its time. A tile of K / 32 steps takes about alone·(steps + overhead) on a CU that
+// it has for itself; a full chip (whose clock the matrix cores' power then sets) gets through one in loaded·(steps +
+// overhead) a CU. Microseconds on 768 x 768 to 2304 x 768 matrices, one and 88 at a time: a 256 tile 47.7 us alone over
+// 24 steps and 122 over 72, a 128 tile 19.0 and 48.2, a 64 tile 10.2 and 29.2. One matrix runs its products best on 64
+// tiles (10 us against 19 and 48), 22 layers gram and poly on 128 (305 + 176 us against 328 + 203 on 256) and update on
+// 256 (489 against 523 on 128).
+int pick_tile(laya_ctx* ctx, Batch& b, bool triangle, bool gram) {
+    const struct { int size, overhead; double alone, loaded; } t[3] = {{256, 7, 1.54, 2.25}, {128, 7, 0.61, 0.7}, {64, 2, 0.40, 0.27}};
     int best = 0;
     double time = 1e30;
     for (int k = 0; k < 3; ++k) {
-        const int units = tile_units(b, t[k].size, triangle);
-        const double rounds = std::max(1.0, (double)units / t[k].slots);
-        const double cost = (rounds < 4 ? std::ceil(rounds) : rounds + 0.5) * t[k].step;
+        tile_units(b, t[k].size, triangle);
+        double total = 0, longest = 0;
+        for (int q = 0; q < b.shapes; ++q) {
+            const Shape& s = b.s[q];
+            const double each = (gram ? s.steps_m : s.steps_n) + t[k].overhead;
+            total += (double)s.count * s.tiles * each;
+            longest = std::max(longest, each);
+        }
+        const double load = total / ctx->cu_count * t[k].loaded, one = longest * t[k].alone;
+        const double cost = load > one ? load + 0.5 * one : one;  // units end unevenly: half a unit beyond the mean
         if (cost < time) {
             time = cost;
-            best = t[k].size;
+            best = k;
         }
     }
-    tile_units(b, best, triangle);
+    tile_units(b, t[best].size, triangle);
     return best;
+}
+
+template <class F> void with_tile(laya_ctx* ctx, Batch& b, bool triangle, bool gram, F&& f) {
+    switch (pick_tile(ctx, b, triangle, gram)) {
+        case 0: return f(T256());
+        case 1: return f(T128());
+        default: return f(T64());
+    }
 }
 
 template <bool POLY>
@@ -403,14 +478,11 @@ void launch_square(laya_ctx* ctx, Batch& b, const _Float16* in, _Float16* out) {
     for (int k = 0; k < b.shapes; ++k)
         flops += (double)b.s[k].count * b.s[k].n * b.s[k].n * (POLY ? b.s[k].n : b.s[k].m);
     ProfileScope scope(ctx, POLY ? "muon_poly" : "muon_gram", flops, 0.0);
-    const int size = pick_tile(ctx, b, true);
-    const dim3 grid(b.units);
-    if (size == 256)
-        LAYA_LAUNCH((muon_square_kernel<T256, POLY>), grid, dim3(512), 0, ctx->stream, b, in, out);
-    else if (size == 128)
-        LAYA_LAUNCH((muon_square_kernel<T128, POLY>), grid, dim3(256), 0, ctx->stream, b, in, out);
-    else
-        LAYA_LAUNCH((muon_square_kernel<T64, POLY>), grid, dim3(256), 0, ctx->stream, b, in, out);
+    with_tile(ctx, b, true, !POLY, [&](auto c) {
+        typedef decltype(c) C;
+        LAYA_LAUNCH((muon_square_kernel<C, POLY>), dim3(b.units), dim3(C::template Tile<false>::THREADS), 0, ctx->stream, b,
+                    in, out);
+    });
     check_launch("muon_square_kernel");
 }
 
@@ -419,14 +491,11 @@ void launch_update(laya_ctx* ctx, Batch& b, const _Float16* X, const _Float16* B
     double flops = 0;
     for (int k = 0; k < b.shapes; ++k) flops += 2.0 * b.s[k].count * b.s[k].n * b.s[k].n * b.s[k].m;
     ProfileScope scope(ctx, "muon_update", flops, 0.0);
-    const int size = pick_tile(ctx, b, false);
-    const dim3 grid(b.units);
-    if (size == 256)
-        LAYA_LAUNCH((muon_update_kernel<T256, LAST>), grid, dim3(512), 0, ctx->stream, b, X, B, out, sink);
-    else if (size == 128)
-        LAYA_LAUNCH((muon_update_kernel<T128, LAST>), grid, dim3(256), 0, ctx->stream, b, X, B, out, sink);
-    else
-        LAYA_LAUNCH((muon_update_kernel<T64, LAST>), grid, dim3(256), 0, ctx->stream, b, X, B, out, sink);
+    with_tile(ctx, b, false, false, [&](auto c) {
+        typedef decltype(c) C;
+        LAYA_LAUNCH((muon_update_kernel<C, LAST>), dim3(b.units), dim3(C::template Tile<true>::THREADS), 0, ctx->stream, b, X,
+                    B, out, sink);
+    });
     check_launch("muon_update_kernel");
 }
 

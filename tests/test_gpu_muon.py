@@ -85,13 +85,13 @@ def test_other_numbers_of_steps(ctx, steps):
             _close(got[k], u[k], steps)
 
 
-def test_many_tiles(ctx):
-    """Enough matrices for each size of tile: 60 of 300 x 400 (128 or 256 wide tiles), in both orders."""
-    for rows, cols in ((300, 400), (400, 300)):
-        u = _matrices(60, rows, cols)
-        got = _orthogonalize(ctx, u)
-        for k in (0, 29, 59):
-            _close(got[k], u[k], 5)
+@pytest.mark.parametrize("count,rows,cols", [(60, 300, 400), (60, 400, 300), (16, 1100, 1056), (10, 1056, 3100)])
+def test_many_tiles(ctx, count, rows, cols):
+    """Enough matrices for each size of tile (256 wide ones in the last two), ending inside them, in both orders."""
+    u = _matrices(count, rows, cols)
+    got = _orthogonalize(ctx, u)
+    for k in (0, count - 1):
+        _close(got[k], u[k], 5)
 
 
 def test_singular_values_gather_near_one(ctx):
