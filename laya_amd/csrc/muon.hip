@@ -239,8 +239,9 @@ typedef Config<256, 4, 1, 2> T256;
 typedef Config<128, 2, 2, 2> T128;
 typedef Config<64, 2, 2, 4> T64;
 
-// The workgroup's tile. Of a run of `many` matrices the tiles of one run on one XCD (workgroups go round the 8), so that its
-// packed rows come into one L2; runs of few spread over all.
+// The workgroup's tile. Of many matrices each one's tiles run on one XCD (workgroups go round the 8), so that its packed
+// rows come into one L2 (22 layers: gram and poly 478 us an iteration against 578 spread); of few, a matrix's tiles go to
+// the XCDs in runs (a layer's four matrices: 109 us an iteration against 118).
 struct Where {
     int shape, index, tile;
 };
@@ -255,8 +256,10 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int u, Where& at) {
         at.index = slot / s.tiles * 8 + ((in + b.s[k].turn) & 7);
         at.tile = slot % s.tiles;
     } else {
-        at.index = in / s.tiles;
-        at.tile = in % s.tiles;
+        const int all = s.count * s.tiles, per = (all + 7) >> 3, t = (in & 7) * per + (in >> 3);
+        if ((in >> 3) >= per || t >= all) return false;
+        at.index = t / s.tiles;
+        at.tile = t % s.tiles;
     }
     return at.index < s.count;
 }
@@ -348,7 +351,9 @@ __global__ __launch_bounds__(C::template Tile<true>::THREADS, C::PER_CU) void mu
     Where at;
     if (!find_tile(b, blockIdx.x, at)) return;
     const Shape& s = b.s[at.shape];
-    const int ti = at.tile / s.across, tj = at.tile % s.across;
+    // Tiles in strips of 6 columns, row by row, so that a run of them shares rows and columns.
+    const int down = s.tiles / s.across, strip = at.tile / (6 * down), wide = min(6, s.across - 6 * strip);
+    const int in_strip = at.tile - strip * 6 * down, ti = in_strip / wide, tj = 6 * strip + in_strip % wide;
     const Operand x{X + s.x0 + at.index * s.x, s.steps_m, s.groups_n}, bb{B + s.ab0 + at.index * s.ab, s.steps_n, s.groups_n};
     typename T::Acc acc;
     T::product(x, bb, ti * T::MG, tj * T::NG, 0, s.steps_n, lds, acc, wave, lane);
@@ -428,7 +433,7 @@ void tile_units(Batch& b, int size, bool triangle) {
         s.tiles = triangle ? s.across * (s.across + 1) / 2 : ceil_div(s.m, size) * s.across;
         s.unit0 = units;
         s.turn = before & 7;
-        units += (b.together ? (s.count + 7) / 8 * 8 : s.count) * s.tiles;
+        units += b.together ? (s.count + 7) / 8 * 8 * s.tiles : (s.count * s.tiles + 7) / 8 * 8;
         before += s.count;
     }
     b.units = units;
