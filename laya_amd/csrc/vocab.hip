@@ -88,7 +88,7 @@ struct PackRows {
 // One workgroup packs 32 rows, scaled so that the largest finite magnitude (a row's own, or the operand's) lies in
 // [2^14, 2^15). Row scales take one read for the magnitudes and one, from the caches, for the pieces. Thread t holds 8
 // columns of row t / 8. T: fp32 or bf16 source.
-template <typename T, int PLANES, bool VEC>
+template <typename T, int PLANES>
 __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
     const int b = blockIdx.x, tid = threadIdx.x, r = tid >> 3, o = tid & 7;
     const int rows = p.count ? (int)*p.count : p.rows;
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
         if (live)
             for (int c = o * 8; c < p.K; c += 64) {
                 float v[8];
-                load8<VEC>(row, c, p.K, v);
+                load8(row, c, p.K, v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) am = max(am, amax_bits(v[i]));
             }
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
     const int steps = (p.K + 31) / 32;
     for (int c = o * 8; c < steps * 32; c += 64) {
         float v[8] = {};
-        if (live) load8<VEC>(row, c, p.K, v);
+        if (live) load8(row, c, p.K, v);
         f16x8 hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -152,10 +152,10 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackRows p) {
 template <typename T>
 __global__ __launch_bounds__(256) void table_amax_kernel(const T* __restrict__ x, size_t n, unsigned* word) {
     constexpr int V = 16 / sizeof(T);
-    typedef T Vec __attribute__((ext_vector_type(V)));
+    typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     unsigned m = 0;
     const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, all = (size_t)gridDim.x * 256;
-    const size_t nv = ((uintptr_t)x & 15u) == 0 ? n / V : 0;
+    const size_t nv = n / V;
     const Vec* xv = reinterpret_cast<const Vec*>(x);
     size_t i = at;
     for (; i + 3 * all < nv; i += 4 * all) {
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void pack_weighted_kernel(const float* __restr
     float v[8] = {};
     if (j < count) {
         const int from = row_of[j];
-        load8<false>(x + (size_t)from * K, c0 + o * 8, K, v);
+        load8(x + (size_t)from * K, c0 + o * 8, K, v);
         const float w = weights ? weights[from] : 1.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= w;
@@ -312,8 +312,34 @@ __global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* _
     }
 }
 
-// One wave a labelled row: the tiles' statistics merged, and the target's logit from W's row itself. The last workgroup to
-// end sums the rows' weighted losses, in their order.
+// Σ w·L of the labelled rows, in an order of its own: one workgroup of N threads.
+template <int N>
+__device__ __forceinline__ void total_loss(const int* row_of, int count, const float* row_loss, const float* weights,
+                                           float scale, float* loss) {
+    __shared__ double red[N / 64];
+    double s = 0.0;
+    for (int k = threadIdx.x; k < count; k += N) {
+        const int r = row_of[k];
+        s += (double)__hip_atomic_load(row_loss + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) *
+             (weights ? (double)weights[r] : 1.0);
+    }
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        for (int k = 0; k < N / 64; ++k) s += red[k];
+        *loss = (float)(s * (double)scale);
+    }
+}
+__global__ __launch_bounds__(1024) void vocab_total_kernel(const int* row_of, const unsigned* words,
+                                                           const float* row_loss, const float* weights, float scale,
+                                                           float* loss) {
+    total_loss<1024>(row_of, (int)words[WORD_COUNT], row_loss, weights, scale, loss);
+}
+
+// One wave a labelled row: the tiles' statistics merged, and the target's logit from W's row itself. With `loss` the last
+// workgroup to end sums the rows' weighted losses.
 template <typename TW>
 __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restrict__ part, int pitch, int tiles,
                                                           unsigned* words, const int* __restrict__ row_of,
@@ -374,23 +400,13 @@ __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restri
     }
     if (!loss) return;
     __shared__ unsigned last;
-    __shared__ double red[4];
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) last = atomicAdd(words + WORD_ENDED, 1u) + 1 == gridDim.x;
     __syncthreads();
     if (!last) return;
     __threadfence();
-    double s = 0.0;
-    for (int k = threadIdx.x; k < count; k += 256) {
-        const int r = row_of[k];
-        s += (double)__hip_atomic_load(row_loss + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) *
-             (weights ? (double)weights[r] : 1.0);
-    }
-    s = wave_sum_d(s);
-    if (lane == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) *loss = (float)(((red[0] + red[1]) + (red[2] + red[3])) * (double)scale);
+    total_loss<256>(row_of, count, row_loss, weights, scale, loss);
 }
 
 struct GradOut {
@@ -489,29 +505,38 @@ struct GradProducts {
     int first;         // the first piece stores, the others add
     int steps_first, units_first;  // the first piece's steps over v and units of dW, which say how dx's sum is split
     int tiles_v, tiles_h;
+    float* dw_part;    // [split][the piece's rows][hidden]: dW's partial sums, when its sum is split
+    int most_e;        // splits that dw_part holds (1: none)
 };
 
-// The ways that dx's sum over a piece is split: those of 1 … MAX_SPLITS whose longest worker ends first. Worker w of G
-// takes units w, w + G, …: dW's ne (each `le` steps), then dx's; the longest is the first of a class of equals.
-__device__ __forceinline__ int dx_splits(int steps_v, int count, int cap_rows, int ne, int tiles_h, int G) {
-    const int tiles_t = (count + TILE - 1) / TILE, le = (count + 31) / 32;
-    const int most = max(1, min(min(MAX_SPLITS, steps_v), cap_rows / max(tiles_t * TILE, 1)));
-    int best = 1;
-    long best_time = 1l << 60;
-    for (int s = 1; s <= most; ++s) {
-        const int units = ne + tiles_t * tiles_h * s, lx = (steps_v + s - 1) / s;
-        long time = 0;
+struct Splits {
+    int x, e;
+};
+// The ways that dx's sum over a piece and dW's over the rows are split: those whose longest worker ends first. Worker w of
+// G takes units w, w + G, …: dW's, then dx's; the longest is the first of a class of equals. A small table has few tiles
+// of dW and, with many rows, long ones: 15320 x 768 x 2304 took 1.6 ms with 27 whole ones, 0.8 with them split.
+// Every wave plans for itself, a pair of splits a lane at a time.
+__device__ __forceinline__ Splits plan_splits(const GradProducts& p, int count, int G, int lane) {
+    const int tiles_t = (count + TILE - 1) / TILE, steps_t = (count + 31) / 32, steps_v = p.steps_first;
+    const int most = p.cap_rows ? max(1, min(min(MAX_SPLITS, steps_v), p.cap_rows / max(tiles_t * TILE, 1))) : 1;
+    const int most_e = max(1, min(p.most_e, steps_t / 8));
+    unsigned long long best = ~0ull;
+    for (int k = lane; k < most * most_e; k += 64) {
+        const int se = k / most + 1, s = k - (se - 1) * most + 1;
+        const int ne = p.units_first * se, le = (steps_t + se - 1) / se + (se > 1 ? 4 : 0);
+        const int units = ne + (p.cap_rows ? tiles_t * p.tiles_h * s : 0), lx = (steps_v + s - 1) / s;
+        unsigned long long time = 0;
         for (int w = 0; w < G; w = w == 0 && ne % G != 0 ? ne % G : G) {
             const int mine = (units - w + G - 1) / G, e = max(0, (ne - w + G - 1) / G);
             // Each unit costs about 24 steps beside its own: the first copies, the stores.
-            time = max(time, (long)e * (le + 24) + (long)(mine - e) * (lx + 24));
+            time = max(time, (unsigned long long)e * (le + 24) + (unsigned long long)(mine - e) * (lx + 24));
         }
-        if (time < best_time) {
-            best_time = time;
-            best = s;
-        }
+        best = min(best, time << 16 | (unsigned)(k & 0xffff));
     }
-    return best;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) best = min(best, (unsigned long long)__shfl_xor((long long)best, o, 64));
+    const int k = (int)(best & 0xffff);
+    return {__builtin_amdgcn_readfirstlane(k % most + 1), __builtin_amdgcn_readfirstlane(k / most + 1)};
 }
 
 // Both products of a piece in one launch.
@@ -524,19 +549,26 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
     const int count = (int)p.words[WORD_COUNT];
     if (count == 0) return;
     const int tiles_t = (count + TILE - 1) / TILE, steps_v = p.g.steps;
-    const int splits = p.cap_rows ? dx_splits(p.steps_first, count, p.cap_rows, p.units_first, p.tiles_h, gridDim.x) : 0;
-    const int units_e = p.tiles_v * p.tiles_h, units = units_e + tiles_t * p.tiles_h * splits;
+    const Splits plan = plan_splits(p, count, gridDim.x, lane);
+    const int splits = p.cap_rows ? plan.x : 0, splits_e = plan.e;
+    const int tiles_e = p.tiles_v * p.tiles_h, units_e = tiles_e * splits_e;
+    const int units = units_e + tiles_t * p.tiles_h * splits, steps_t = (count + 31) / 32;
     const int e_wx = -(G_SCALE + pair_scale_exp(p.words[WORD_WX])), e_w = -(G_SCALE + pair_scale_exp(p.words[WORD_W]));
     p.g.groups = (count + 31) / 32;
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.words[WORD_SPLITS] = splits;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.words[WORD_SPLITS] = splits;
+        p.words[WORD_SPLITS_E] = splits_e;
+    }
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
         if (u >= units) continue;
         typename TE::Acc acc;
         if (u < units_e) {
-            const int tv = u / p.tiles_h, th = u - tv * p.tiles_h;
-            TE::product(p.g, p.wx, tv * TE::MG, th * TE::NG, 0, (count + 31) / 32, lds, acc, wave, lane);
+            const int se = u / tiles_e, in = u - se * tiles_e, tv = in / p.tiles_h, th = in - tv * p.tiles_h;
+            const int s0 = (int)((long)steps_t * se / splits_e), s1 = (int)((long)steps_t * (se + 1) / splits_e);
+            TE::product(p.g, p.wx, tv * TE::MG, th * TE::NG, s0, s1, lds, acc, wave, lane);
+            float* out = splits_e > 1 ? p.dw_part + (size_t)se * p.vocab * p.hidden : p.dW;
             const int v = tv * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -545,15 +577,15 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const bool in = h + 16 * j < p.hidden && v + 16 * i + r < p.vocab;
-                        old[j][r] = in ? p.dW[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] : 0.0f;
+                        const bool in = splits_e == 1 && h + 16 * j < p.hidden && v + 16 * i + r < p.vocab;
+                        old[j][r] = in ? out[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] : 0.0f;
                     }
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (h + 16 * j < p.hidden && v + 16 * i + r < p.vocab)
-                            p.dW[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] =
+                            out[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] =
                                 old[j][r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_wx) * p.scale;
             }
         } else {
@@ -583,6 +615,18 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
             }
         }
     }
+}
+
+// dW += Σ over the splits of its sum, where it was split.
+__global__ __launch_bounds__(256) void vocab_dw_kernel(const float* __restrict__ part, const unsigned* words, size_t n,
+                                                       float* __restrict__ dW) {
+    const int splits = (int)words[WORD_SPLITS_E];
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (splits < 2 || i >= n) return;
+    float s = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += part[k * n + i];
+    dW[i] += s;
 }
 
 // dx_r = w_r·scale·Σ over the splits, 0 for rows without a label.
@@ -619,11 +663,7 @@ long pad_tile(long n) { return (n + TILE - 1) / TILE * TILE; }
 
 template <typename T, int PLANES>
 void launch_pack(laya_ctx* ctx, const PackRows& p, int blocks) {
-    const bool vec = p.K % 8 == 0 && ((uintptr_t)p.src & 15u) == 0;
-    if (vec)
-        LAYA_LAUNCH((pack_rows_kernel<T, PLANES, true>), dim3(blocks), dim3(256), 0, ctx->stream, p);
-    else
-        LAYA_LAUNCH((pack_rows_kernel<T, PLANES, false>), dim3(blocks), dim3(256), 0, ctx->stream, p);
+    LAYA_LAUNCH((pack_rows_kernel<T, PLANES>), dim3(blocks), dim3(256), 0, ctx->stream, p);
     check_launch("pack_rows_kernel");
 }
 
@@ -694,14 +734,24 @@ int workgroups(const laya_ctx* ctx) { return std::max(8, ctx->cu_count / 8 * 8);
 
 void vocab_merge(laya_ctx* ctx, const VocabArgs& a, const float2* part, int pitch, int tiles, unsigned* words,
                  const int* row_of, float* row_loss, float* lse, float* loss) {
+    // The total by the last workgroup saves a launch (4 of 52 µs at 19 rows), but its fences cost 0.07 µs a workgroup, one
+    // after another: 250 µs at 13871 rows, where a launch of its own takes 6.
+    const bool own = a.rows > VOCAB_FEW;
     const dim3 grid((a.rows + 3) / 4);
     if (a.W16)
         LAYA_LAUNCH(vocab_merge_kernel<__bf16>, grid, dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
-                    a.targets, a.x, a.W16, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale, loss);
+                    a.targets, a.x, a.W16, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale,
+                    own ? nullptr : loss);
     else
         LAYA_LAUNCH(vocab_merge_kernel<float>, grid, dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
-                    a.targets, a.x, a.W, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale, loss);
+                    a.targets, a.x, a.W, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale,
+                    own ? nullptr : loss);
     check_launch("vocab_merge_kernel");
+    if (loss && own) {
+        LAYA_LAUNCH(vocab_total_kernel, dim3(1), dim3(1024), 0, ctx->stream, row_of, words, row_loss, a.row_weights,
+                    a.scale, loss);
+        check_launch("vocab_total_kernel");
+    }
 }
 
 void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count) {
@@ -760,9 +810,13 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
     const int piece = piece_rows(ctx, a.vocab, (size_t)steps_h * 64 * planes + (size_t)steps_t * 128 + 8 + (db ? 16 * tiles_t : 0),
                                  4 * halves(a.rows, a.hidden, 2) + 16 * (size_t)pitch +
                                      (dx ? 4 * (size_t)cap_rows * a.hidden : 0));
+    // dW's partial sums: a table of few tiles, whole in one piece, takes as many splits as fill the chip twice.
+    const int tiles_e = dW && piece >= a.vocab ? (a.vocab + TILE - 1) / TILE * tiles_h : 0;
+    const int most_e =
+        tiles_e && !ctx->cap ? std::max(1, std::min({MAX_SPLITS, 2 * workgroups(ctx) / tiles_e, steps_t / 8})) : 1;
     unsigned* words;
     int *row_of, *place, *ex, *ew;
-    float *padded, *part, *db_part;
+    float *padded, *part, *db_part, *dw_part;
     _Float16 *xp, *xt, *wp, *gp;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
         ws.take(words, WORDS);
@@ -777,6 +831,7 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
         ws.take(gp, halves(a.rows, piece, 2));
         ws.take(part, dx ? (size_t)cap_rows * a.hidden : 0);
         ws.take(db_part, db ? (size_t)tiles_t * 4 * piece : 0);
+        ws.take(dw_part, most_e > 1 ? (size_t)most_e * a.vocab * a.hidden : 0);
     });
     if (!db) db_part = nullptr;
     LAYA_LAUNCH(label_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, a.targets, a.rows, a.vocab, row_of, place, words,
@@ -827,6 +882,8 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
         q.units_first = units_e;
         q.tiles_v = dW ? tiles_v : 0;
         q.tiles_h = tiles_h;
+        q.dw_part = dw_part;
+        q.most_e = most_e;
         if (dx || dW) {
             ProfileScope scope(ctx, "vocab_products", ((dx ? 2.0 : 0.0) + (dW ? 2.0 : 0.0)) * a.rows * a.hidden * n, 0.0);
             if (a.W16)
@@ -834,6 +891,12 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
             else
                 LAYA_LAUNCH(vocab_products_kernel<2>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, q);
             check_launch("vocab_products_kernel");
+        }
+        if (most_e > 1) {
+            const size_t n_e = (size_t)a.vocab * a.hidden;
+            LAYA_LAUNCH(vocab_dw_kernel, dim3((unsigned)((n_e + 255) / 256)), dim3(256), 0, ctx->stream, dw_part, words,
+                        n_e, dW);
+            check_launch("vocab_dw_kernel");
         }
         if (db) {
             LAYA_LAUNCH(vocab_db_kernel, dim3((n + 255) / 256), dim3(256), 0, ctx->stream, db_part, piece, words, n,

@@ -9,33 +9,32 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr int VOCAB_FEW = 256;  // rows that the few-row kernels take at most
 
 // Words of a call: labelled rows, targets outside the vocabulary, bits of max|w_t·x_t| and of max|W|, the ways that dx's
-// sum is split, workgroups that have ended.
-enum : int { WORD_COUNT, WORD_BAD, WORD_WX, WORD_W, WORD_SPLITS, WORD_ENDED, WORDS };
+// sum and dW's are split, workgroups that have ended.
+enum : int { WORD_COUNT, WORD_BAD, WORD_WX, WORD_W, WORD_SPLITS, WORD_SPLITS_E, WORD_ENDED, WORDS };
 
-// Eight consecutive values of a row from column c, zeros behind K. VEC: rows start on 16 bytes and K is a multiple of 8.
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* row, int c, int K, float (&v)[8]) {
-    if constexpr (VEC) {
-        const f32x4 zero = {};
-        const f32x4 a = c < K ? *reinterpret_cast<const f32x4*>(row + c) : zero;
-        const f32x4 b = c < K ? *reinterpret_cast<const f32x4*>(row + c + 4) : zero;
+// Vector loads that ask for the elements' own alignment alone: the hardware takes them at any, so that a table of an odd
+// width, or one that starts inside another array, reads as fast as an aligned one.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+
+__device__ __forceinline__ void load8(const float* at, float (&v)[8]) {
+    const f32x4_any a = *reinterpret_cast<const f32x4_any*>(at), b = *reinterpret_cast<const f32x4_any*>(at + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < K ? row[c + i] : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
     }
 }
-template <bool VEC>
-__device__ __forceinline__ void load8(const __bf16* row, int c, int K, float (&v)[8]) {
-    if constexpr (VEC) {
-        const bf16x8 zero = {};
-        const bf16x8 a = c < K ? *reinterpret_cast<const bf16x8*>(row + c) : zero;
+__device__ __forceinline__ void load8(const __bf16* at, float (&v)[8]) {
+    const bf16x8_any a = *reinterpret_cast<const bf16x8_any*>(at);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+}
+// Eight consecutive values of a row from column c, zeros behind K.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int c, int K, float (&v)[8]) {
+    if (c + 8 <= K) {
+        load8(row + c, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = c + i < K ? (float)row[c + i] : 0.0f;

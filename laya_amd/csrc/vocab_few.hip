@@ -79,8 +79,7 @@ struct Prepare {
     float *row_loss, *lse;              // of the forward (null in the backward)
 };
 
-// One workgroup a step of 32 columns of x; each finds the rows' scales for itself. VEC: rows of float4s.
-template <bool VEC>
+// One workgroup a step of 32 columns of x; each finds the rows' scales for itself.
 __global__ __launch_bounds__(1024) void few_prepare_kernel(Prepare p) {
     __shared__ int row_of[VOCAB_FEW], row_exp[VOCAB_FEW];
     __shared__ float tile[VOCAB_FEW][33];
@@ -100,13 +99,10 @@ __global__ __launch_bounds__(1024) void few_prepare_kernel(Prepare p) {
         unsigned m = 0;
         if (j < count) {
             const float* row = p.x + (size_t)row_of[j] * p.hidden;
-            if constexpr (VEC) {
+            int c = 4 * (tid & 15);
 #pragma unroll 8
-                for (int c = 4 * (tid & 15); c < p.hidden; c += 64)
-                    m = max(m, amax_bits4(*reinterpret_cast<const f32x4*>(row + c)));
-            } else {
-                for (int c = tid & 15; c < p.hidden; c += 16) m = max(m, amax_bits(row[c]));
-            }
+            for (; c + 4 <= p.hidden; c += 64) m = max(m, amax_bits4(*reinterpret_cast<const f32x4_any*>(row + c)));
+            for (; c < p.hidden; ++c) m = max(m, amax_bits(row[c]));  // a piece of four
         }
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
@@ -229,31 +225,13 @@ struct FewLogits {
     float scale;
 };
 
-
-// load8 as two loads (fp32) or one (bf16) whatever the column (aligned rows of a multiple of 8); the caller clears what lies
-// behind K.
-__device__ __forceinline__ void load8_always(const float* row, int c, int K, float (&v)[8]) {
-    const int at = c < K ? c : 0;
-    const f32x4 a = *reinterpret_cast<const f32x4*>(row + at), b = *reinterpret_cast<const f32x4*>(row + at + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = a[i];
-        v[4 + i] = b[i];
-    }
-}
-__device__ __forceinline__ void load8_always(const __bf16* row, int c, int K, float (&v)[8]) {
-    const bf16x8 a = *reinterpret_cast<const bf16x8*>(row + (c < K ? c : 0));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-}
-
 // Blocks of 16 rows of W a wave takes: with many rows of x it is their reads from LDS that two blocks share.
 constexpr int wave_blocks(int nb) { return nb >= 8 ? 2 : 1; }
 // Steps of a ring: what is under way of W waits in registers.
 constexpr int ring_of(int nb) { return nb >= 12 ? 3 : 4; }
 
 // A workgroup is as many waves, WAVES at least, as spread the table's blocks of 16 rows evenly over the CUs.
-template <int NB, typename TW, bool VEC, bool GRAD, int WAVES>
+template <int NB, typename TW, bool GRAD, int WAVES>
 __global__ __launch_bounds__(1024 / wave_blocks(NB), 1) void few_logits_kernel(FewLogits p) {
     constexpr int PW = sizeof(TW) == 2 ? 1 : 2, VB = wave_blocks(NB), RING = ring_of(NB);
     constexpr int LOADS = VB * (sizeof(TW) == 2 ? 1 : 2);
@@ -268,14 +246,9 @@ __global__ __launch_bounds__(1024 / wave_blocks(NB), 1) void few_logits_kernel(F
         row[i] = static_cast<const TW*>(p.W) + (size_t)min(v0 + 16 * i + (lane & 15), p.vocab - 1) * p.hidden;
     const S x(p.x_rows, lds, wave, lane, steps);
     auto load = [&](int s, float (&w)[VB][8]) {
-        const int c = 32 * s + 8 * (lane >> 4);
+        const int c = min(32 * s + 8 * (lane >> 4), p.hidden - 8);  // the last 8 also for what reaches behind them
 #pragma unroll
-        for (int i = 0; i < VB; ++i) {
-            if constexpr (VEC)
-                load8_always(row[i], c, p.hidden, w[i]);
-            else
-                load8<false>(row[i], c, p.hidden, w[i]);
-        }
+        for (int i = 0; i < VB; ++i) load8(row[i] + c, w[i]);
     };
     float w[RING][VB][8];
     int e = 126;           // of the wave's scale
@@ -294,18 +267,23 @@ __global__ __launch_bounds__(1024 / wave_blocks(NB), 1) void few_logits_kernel(F
     auto step = [&](int s, auto slot) {
         constexpr int K = decltype(slot)::value;
         // Step s's copies have landed for every wave, and step s − 1 is read by all: its slot is free.
-        if constexpr (VEC)
-            wait_step<RING, S::PER, LOADS>();
-        else
-            packed::wait_copies<0>();
+        wait_step<RING, S::PER, LOADS>();
         x.start(s + RING - 1);
         load(s + RING - 1, w[(K + RING - 1) % RING]);
         __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
-        if (VEC && 32 * s + 8 * (lane >> 4) >= p.hidden)
+        if (32 * s + 32 > p.hidden) {  // the last step: what was loaded from the row's end moves to its place
+            const int left = p.hidden - 32 * s - 8 * (lane >> 4);
+            for (int q = p.hidden & 7; q > 0 && q < 8; ++q)
+#pragma unroll
+                for (int i = 0; i < VB; ++i)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (left > 0 && left < 8) w[K][i][k] = k < 7 ? w[K][i][k + 1 < 8 ? k + 1 : 7] : 0.0f;
 #pragma unroll
             for (int i = 0; i < VB; ++i)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) w[K][i][k] = 0.0f;
+                for (int k = 0; k < 8; ++k) w[K][i][k] = left > 0 ? w[K][i][k] : 0.0f;
+        }
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < VB; ++i)
@@ -479,10 +457,10 @@ struct FewDx {
 };
 
 // A workgroup: 256 columns of W over a slice of the vocabulary; a wave 32 of them, block i the columns 2·n + i, so that a
-// lane's two blocks come with one load a row (PAIR: rows of pairs).
-template <int NB, typename TW, bool PAIR>
+// lane's two blocks come with one load a row.
+template <int NB, typename TW>
 __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
-    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = PAIR ? 8 : 16, RING = 4;
+    constexpr int PW = sizeof(TW) == 2 ? 1 : 2, LOADS = 8, RING = 4;
     typedef Stream<2 * NB, 8, RING> S;
     __shared__ __attribute__((aligned(16))) _Float16 lds[RING * S::STEP];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -490,24 +468,19 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
     const int h0 = blockIdx.x * 256 + wave * 32;
     const TW* W = static_cast<const TW*>(p.W);
     const S g(p.g_rows + (size_t)first * S::STEP, lds, wave, lane, steps);
-    int col[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) col[i] = min(h0 + 2 * (lane & 15) + i, p.hidden - (PAIR ? 2 - i : 1));
+    // The last pair for what reaches behind it; of an odd width its second is the last column.
+    const int col = min(h0 + 2 * (lane & 15), p.hidden - 2);
+    const bool second = h0 + 2 * (lane & 15) == p.hidden - 1;
     // Rows behind the vocabulary read its last: G is zero there.
     auto load = [&](int s, float (&w)[2][8]) {
         const int v = 32 * (first + min(s, steps - 1)) + 8 * (lane >> 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const TW* at = W + (size_t)min(v + e, p.vocab - 1) * p.hidden;
-            if constexpr (PAIR) {
-                typedef TW Pair __attribute__((ext_vector_type(2)));
-                const Pair both = *reinterpret_cast<const Pair*>(at + col[0]);
-                w[0][e] = (float)both[0];
-                w[1][e] = (float)both[1];
-            } else {
-                w[0][e] = (float)at[col[0]];
-                w[1][e] = (float)at[col[1]];
-            }
+            typedef TW Pair __attribute__((ext_vector_type(2), aligned(sizeof(TW))));
+            const Pair both = *reinterpret_cast<const Pair*>(at + col);
+            w[0][e] = (float)both[0];
+            w[1][e] = (float)both[1];
         }
     };
     const int ew = pair_scale_exp(p.words[WORD_W]);
@@ -530,6 +503,9 @@ __global__ __launch_bounds__(512, 1) void few_dx_kernel(FewDx p) {
         load(s + RING - 1, w[(K + RING - 1) % RING]);
         __builtin_amdgcn_sched_barrier(0);  // not to the step's end, where the scheduler would have them
         f16x8 a[2][2], b[2][2];
+        if (second)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[K][0][e] = w[K][1][e];
         split8(w[K][0], sc, a[0]);
         split8(w[K][1], sc, a[1]);
         const _Float16* gs = lds + K * S::STEP;
@@ -599,7 +575,7 @@ struct FewDw {
 
 // A wave: 16 rows of dW, their G in registers, HB blocks of 16 columns at a time. A chunk's x comes through LDS, its dW to
 // registers, both started while the chunk before is computed.
-template <int STEPS_T, bool VEC>
+template <int STEPS_T>
 __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
     if (p.words[WORD_COUNT] == 0) return;
     constexpr int HB = STEPS_T == 1 ? 8 : STEPS_T <= 4 ? 4 : 2;
@@ -620,11 +596,11 @@ __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
     auto fetch = [&](int chunk, int k) {
         const int h = 16 * (chunk * HB + k) + 4 * (lane >> 4);
         f32x4 o = {};
-        if constexpr (VEC) {
-            if (h < p.hidden) o = *reinterpret_cast<const f32x4*>(row + h);
-        } else {
+        if (h + 4 <= p.hidden) {
+            o = *reinterpret_cast<const f32x4_any*>(row + h);
+        } else if (h < p.hidden) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 3; ++e)
                 if (h + e < p.hidden) o[e] = row[h + e];
         }
         return o;
@@ -658,11 +634,11 @@ __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
             for (int r = 0; r < 4; ++r) now[k][r] += __builtin_amdgcn_ldexpf(sum[r], e) * p.scale;
             const int h = 16 * (c * HB + k) + 4 * (lane >> 4);
             if (!live) continue;
-            if constexpr (VEC) {
-                if (h < p.hidden) *reinterpret_cast<f32x4*>(row + h) = now[k];
-            } else {
+            if (h + 4 <= p.hidden) {
+                *reinterpret_cast<f32x4_any*>(row + h) = now[k];
+            } else if (h < p.hidden) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int e = 0; e < 3; ++e)
                     if (h + e < p.hidden) row[h + e] = now[k][e];
             }
         }
@@ -671,13 +647,8 @@ __global__ __launch_bounds__(1024, 1) void few_dw_kernel(FewDw p) {
 
 // ------------------------------------------------------------------------------------------ launches
 
-// Whether W's rows take 16-byte loads; without, the kernels of 8 blocks serve every number of rows.
-bool aligned_table(const VocabArgs& a) {
-    return a.hidden % 8 == 0 && ((a.W16 ? (uintptr_t)a.W16 : (uintptr_t)a.W) & 15u) == 0;
-}
 int blocks_of(const VocabArgs& a) {
     const int b = (a.rows + 15) / 16;
-    if (!aligned_table(a)) return 8;
     return b <= 6 ? b : b <= 8 ? 8 : b <= 10 ? 10 : b <= 12 ? 12 : 16;
 }
 
@@ -704,10 +675,7 @@ template <class F> void with_blocks(int nb, F&& f) {
 }
 
 void launch_prepare(laya_ctx* ctx, const Prepare& p, int steps) {
-    if (p.hidden % 4 == 0 && ((uintptr_t)p.x & 15u) == 0)
-        LAYA_LAUNCH(few_prepare_kernel<true>, dim3(steps), dim3(1024), 0, ctx->stream, p);
-    else
-        LAYA_LAUNCH(few_prepare_kernel<false>, dim3(steps), dim3(1024), 0, ctx->stream, p);
+    LAYA_LAUNCH(few_prepare_kernel, dim3(steps), dim3(1024), 0, ctx->stream, p);
     check_launch("few_prepare_kernel");
 }
 
@@ -717,25 +685,18 @@ void launch_logits(laya_ctx* ctx, const VocabArgs& a, const FewLogits& p, int nb
     const dim3 grid((p.blocks_v + waves * each - 1) / (waves * each)), block(64 * waves);
     ProfileScope scope(ctx, "vocab_few_logits", 2.0 * a.rows * a.hidden * a.vocab,
                        (a.W16 ? 2.0 : 4.0) * a.hidden * a.vocab);
-    if (!aligned_table(a)) {
-        if (a.W16)
-            LAYA_LAUNCH((few_logits_kernel<8, __bf16, false, GRAD, 4>), grid, block, 0, ctx->stream, p);
+    with_blocks(nb, [&](auto n) {
+        constexpr int NB = decltype(n)::value;
+        constexpr int MANY = wave_blocks(NB) == 2 ? 6 : 8;
+        if (a.W16 && waves >= MANY)
+            LAYA_LAUNCH((few_logits_kernel<NB, __bf16, GRAD, MANY>), grid, block, 0, ctx->stream, p);
+        else if (a.W16)
+            LAYA_LAUNCH((few_logits_kernel<NB, __bf16, GRAD, 4>), grid, block, 0, ctx->stream, p);
+        else if (waves >= MANY)
+            LAYA_LAUNCH((few_logits_kernel<NB, float, GRAD, MANY>), grid, block, 0, ctx->stream, p);
         else
-            LAYA_LAUNCH((few_logits_kernel<8, float, false, GRAD, 4>), grid, block, 0, ctx->stream, p);
-    } else {
-        with_blocks(nb, [&](auto n) {
-            constexpr int NB = decltype(n)::value;
-            constexpr int MANY = wave_blocks(NB) == 2 ? 6 : 8;
-            if (a.W16 && waves >= MANY)
-                LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, MANY>), grid, block, 0, ctx->stream, p);
-            else if (a.W16)
-                LAYA_LAUNCH((few_logits_kernel<NB, __bf16, true, GRAD, 4>), grid, block, 0, ctx->stream, p);
-            else if (waves >= MANY)
-                LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, MANY>), grid, block, 0, ctx->stream, p);
-            else
-                LAYA_LAUNCH((few_logits_kernel<NB, float, true, GRAD, 4>), grid, block, 0, ctx->stream, p);
-        });
-    }
+            LAYA_LAUNCH((few_logits_kernel<NB, float, GRAD, 4>), grid, block, 0, ctx->stream, p);
+    });
     check_launch("few_logits_kernel");
 }
 
@@ -745,14 +706,10 @@ void launch_dx(laya_ctx* ctx, const VocabArgs& a, const FewDx& p, int slices, in
                        (a.W16 ? 2.0 : 4.0) * a.hidden * a.vocab);
     with_blocks(nb, [&](auto n) {
         constexpr int NB = decltype(n)::value;
-        if (a.W16 && aligned_table(a))
-            LAYA_LAUNCH((few_dx_kernel<NB, __bf16, true>), grid, block, 0, ctx->stream, p);
-        else if (a.W16)
-            LAYA_LAUNCH((few_dx_kernel<NB, __bf16, false>), grid, block, 0, ctx->stream, p);
-        else if (aligned_table(a))
-            LAYA_LAUNCH((few_dx_kernel<NB, float, true>), grid, block, 0, ctx->stream, p);
+        if (a.W16)
+            LAYA_LAUNCH((few_dx_kernel<NB, __bf16>), grid, block, 0, ctx->stream, p);
         else
-            LAYA_LAUNCH((few_dx_kernel<NB, float, false>), grid, block, 0, ctx->stream, p);
+            LAYA_LAUNCH((few_dx_kernel<NB, float>), grid, block, 0, ctx->stream, p);
     });
     check_launch("few_dx_kernel");
 }
@@ -761,16 +718,13 @@ template <int STEPS_T>
 void launch_dw(laya_ctx* ctx, const VocabArgs& a, const FewDw& p, int waves) {
     const dim3 grid((p.blocks_v + waves - 1) / waves), block(64 * waves);
     ProfileScope scope(ctx, "vocab_few_dw", 2.0 * a.rows * a.hidden * a.vocab, 8.0 * a.hidden * a.vocab);
-    if (a.hidden % 16 == 0 && ((uintptr_t)p.dW & 15u) == 0)
-        LAYA_LAUNCH((few_dw_kernel<STEPS_T, true>), grid, block, 0, ctx->stream, p);
-    else
-        LAYA_LAUNCH((few_dw_kernel<STEPS_T, false>), grid, block, 0, ctx->stream, p);
+    LAYA_LAUNCH(few_dw_kernel<STEPS_T>, grid, block, 0, ctx->stream, p);
     check_launch("few_dw_kernel");
 }
 
 }  // namespace
 
-bool vocab_few_rows(const VocabArgs& a) { return a.rows <= (aligned_table(a) ? VOCAB_FEW : 128); }
+bool vocab_few_rows(const VocabArgs& a) { return a.rows <= VOCAB_FEW && a.hidden >= 8; }  // rows of whole octets
 
 void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count) {
     const int nb = blocks_of(a), pitch = 16 * nb, steps = packed::steps_of(a.hidden);

@@ -127,8 +127,7 @@ def _check(got, want, tol, names=("row_loss", "lse", "loss", "dx", "dW", "db")):
         assert not np.any(over | ~np.isfinite(off)), (k, float(np.max(off)), float(np.max(off / np.maximum(tol[k], 1e-300))))
 
 
-# Rows either side of a block of 16, of the few-row kernels' counts, of their last (256; 128 where rows of W are not
-# multiples of 8) and of whole tiles; widths and vocabularies that end inside a fragment, a step and a tile.
+# Rows either side of a block of 16, of the few-row kernels' counts, of their last (256) and of whole tiles; widths and vocabularies that end inside a fragment, a step and a tile.
 SHAPES = [(1, 64, 300), (1, 1, 1), (2, 7, 2), (15, 32, 31), (16, 33, 32), (17, 96, 257), (33, 40, 500), (64, 72, 1000),
           (77, 136, 1300), (96, 48, 333), (127, 30, 70), (128, 64, 400), (129, 30, 70), (129, 64, 800), (160, 64, 520),
           (192, 40, 300), (193, 64, 300), (256, 24, 290), (257, 64, 300), (300, 100, 777), (513, 33, 1025), (700, 264, 600)]
@@ -143,6 +142,33 @@ def test_matches_the_definition(ctx, rows, hidden, vocab, bf16):
     got = _run(ctx, p)
     assert got["bad"] == 0
     _check(got, want, tol)
+
+
+@pytest.mark.parametrize("hidden", [7, 8, 9, 11, 31, 37, 66, 71, 129])
+@pytest.mark.parametrize("rows", [13, 90, 210])
+def test_widths_that_end_inside_a_load(ctx, rows, hidden):
+    """A row of eight, four and two at a time: its last loads start where a whole one still fits."""
+    for bf16 in (False, True):
+        p = _problem(rows, hidden, 350, weighted=True, bf16=bf16)
+        want, tol = _exact(p)
+        _check(_run(ctx, p), want, tol)
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(1500, 40, 90), (2100, 264, 300), (5000, 33, 260)])
+@pytest.mark.parametrize("labelled", [1.0, 0.1])
+def test_many_rows_over_a_small_table(ctx, rows, hidden, vocab, labelled):
+    """Few tiles of dW, whose sum over the rows is split, or not, as the labelled rows make it; dW adds to what is there."""
+    p = _problem(rows, hidden, vocab, labelled=labelled, weighted=True)
+    start = {"dW": np.random.default_rng(2).standard_normal((vocab, hidden)).astype(np.float32),
+             "db": np.zeros(vocab, np.float32)}
+    want, tol = _exact(p)
+    want["dW"] = want["dW"] + start["dW"]
+    tol["dW"] = tol["dW"] + 2 * U * np.abs(want["dW"])
+    got = _run(ctx, p, start=start)
+    _check(got, want, tol)
+    again = _run(ctx, p, start=start)
+    for k in ("dx", "dW", "db"):
+        np.testing.assert_array_equal(got[k], again[k])
 
 
 @pytest.mark.parametrize("rows,labelled", [(40, 0.5), (250, 0.1), (300, 0.6), (900, 0.15), (600, 0.003), (20, 0.0), (400, 0.0)])
