@@ -20,10 +20,21 @@ namespace {
 
 using namespace packed;
 
-constexpr int TILE = 256;            // logits, G and both gradient products run on 256 x 256 tiles
+constexpr int TILE = 256;            // what rows are padded to: the larger of the products' tiles
 constexpr int G_SCALE = 14;          // |G| ≤ 1
-constexpr int MAX_SPLITS = 16;       // ways of dx's sum over a piece of the vocabulary
+constexpr int MAX_SPLITS = 32;       // ways of dx's sum over a piece of the vocabulary, and of dW's over the rows
 constexpr size_t PIECE_BYTES = (size_t)3 << 30;  // of packed table and G that a piece of the vocabulary may take
+
+// Square tiles of the products and how many workgroups share a CU.
+template <int SIZE_, int WAVES_N, int PER_CU_>
+struct Config {
+    static constexpr int SIZE = SIZE_, WN = WAVES_N, PER_CU = PER_CU_, BM = SIZE / 32, BN = SIZE / 16 / WN;
+    static constexpr int THREADS = 128 * WN, WM_ROWS = SIZE / 2, WN_COLS = SIZE / WN;
+    template <int PA, int PB, bool TA = false, bool TB = false>
+    using Tile = packed::Tile<2, WN, BM, BN, PA, PB, TA, TB, 2>;
+};
+typedef Config<256, 4, 1> T256;
+typedef Config<128, 2, 2> T128;
 
 // ------------------------------------------------------------------------------------------- labels
 
@@ -231,7 +242,6 @@ struct Logits {
     const float* bias;         // padded to whole tiles, −∞ behind the piece
     const unsigned* words;
     int v0, vocab;             // the piece's first row, its rows
-    int tiles_v;
 };
 
 // Tiles are taken in groups of 8 vocabulary tiles, all token tiles of a group before the next: 32 tiles in a row, what
@@ -243,48 +253,49 @@ __device__ __forceinline__ void grouped_tile(int u, int tiles_v, int tiles_t, in
 }
 
 // The wave's logits from its accumulators, in place; `v` and `t`: the first of the wave's rows and columns.
-template <class Acc>
-__device__ __forceinline__ void to_logits(const Logits& p, Acc& acc, int v, int t, int lane) {
-    int ex[4];
+template <int BM, int BN>
+__device__ __forceinline__ void to_logits(const Logits& p, f32x4 (&acc)[BM][BN], int v, int t, int lane) {
+    int ex[BN];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ex[j] = p.ex[t + 16 * j + (lane & 15)];
+    for (int j = 0; j < BN; ++j) ex[j] = p.ex[t + 16 * j + (lane & 15)];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < BM; ++i) {
         const int at = v + 16 * i + 4 * (lane >> 4);
         const int4 ew = *reinterpret_cast<const int4*>(p.ew + at);
         const f32x4 b = *reinterpret_cast<const f32x4*>(p.bias + at);
         const int e[4] = {ew.x, ew.y, ew.z, ew.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < BN; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_ldexpf(acc[i][j][r], -(e[r] + ex[j])) + b[r];
     }
 }
 
 // Each tile's maximum and Σ exp(z − maximum) for every row (token): part[tile_v][t].
-template <int PW>
-__global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* __restrict__ part, int pitch) {
-    typedef Tile<2, 4, 8, 4, PW, 2> T;
+template <class C, int PW>
+__global__ __launch_bounds__(C::THREADS, C::PER_CU) void vocab_stats_kernel(Logits p, float2* __restrict__ part, int pitch) {
+    typedef typename C::template Tile<PW, 2> T;
+    constexpr int SIZE = C::SIZE, BM = C::BM, BN = C::BN;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / C::WN, wn = wave % C::WN;
     const int count = (int)p.words[WORD_COUNT];
-    const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
+    const int tiles_t = (count + SIZE - 1) / SIZE, tiles_v = (p.vocab + SIZE - 1) / SIZE, units = tiles_v * tiles_t;
     p.x.groups = (count + 31) / 32;
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
         if (u >= units) continue;
         int tv, tt;
-        grouped_tile(u, p.tiles_v, tiles_t, tv, tt);
+        grouped_tile(u, tiles_v, tiles_t, tv, tt);
         typename T::Acc acc;
         T::product(p.W, p.x, tv * T::MG, tt * T::NG, 0, p.W.steps, lds, acc, wave, lane);
-        to_logits(p, acc, tv * TILE + wm * 128, tt * TILE + wn * 64, lane);
+        to_logits(p, acc, tv * SIZE + wm * C::WM_ROWS, tt * SIZE + wn * C::WN_COLS, lane);
         float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < BN; ++j) {
             float m = -__builtin_inff();
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < BM; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
             m = fmaxf(m, __shfl_xor(m, 16, 64));
@@ -292,21 +303,21 @@ __global__ __launch_bounds__(512, 1) void vocab_stats_kernel(Logits p, float2* _
             const float at = m == -__builtin_inff() ? 0.0f : m;
             float s[4] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < BM; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[r] += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * LOG2E);
             float sum = (s[0] + s[1]) + (s[2] + s[3]);
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
-            if (lane < 16) red[wm * TILE + wn * 64 + 16 * j + lane] = make_float2(m, sum);
+            if (lane < 16) red[wm * SIZE + wn * C::WN_COLS + 16 * j + lane] = make_float2(m, sum);
         }
         __syncthreads();
-        if (threadIdx.x < TILE) {
-            const float2 a = red[threadIdx.x], b = red[TILE + threadIdx.x];
+        if (threadIdx.x < SIZE) {
+            const float2 a = red[threadIdx.x], b = red[SIZE + threadIdx.x];
             const float m = fmaxf(a.x, b.x), at = m == -__builtin_inff() ? 0.0f : m;
             const float sum = a.y * __builtin_amdgcn_exp2f((a.x - at) * LOG2E) +
                               b.y * __builtin_amdgcn_exp2f((b.x - at) * LOG2E);
-            part[(size_t)(p.v0 / TILE + tv) * pitch + tt * TILE + threadIdx.x] = make_float2(m, sum);
+            part[(size_t)(p.v0 / SIZE + tv) * pitch + tt * SIZE + threadIdx.x] = make_float2(m, sum);
         }
         __syncthreads();
     }
@@ -419,27 +430,28 @@ struct GradOut {
 };
 
 // A piece's G, packed as it lies in the accumulators (a lane has four v of one t in a row).
-template <int PW, bool DB>
-__global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g) {
-    typedef Tile<2, 4, 8, 4, PW, 2> T;
+template <class C, int PW, bool DB>
+__global__ __launch_bounds__(C::THREADS, C::PER_CU) void vocab_grad_kernel(Logits p, GradOut g) {
+    typedef typename C::template Tile<PW, 2> T;
+    constexpr int SIZE = C::SIZE, BM = C::BM, BN = C::BN;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / C::WN, wn = wave % C::WN;
     const int count = (int)p.words[WORD_COUNT];
-    const int tiles_t = (count + TILE - 1) / TILE, units = p.tiles_v * tiles_t;
+    const int tiles_t = (count + SIZE - 1) / SIZE, tiles_v = (p.vocab + SIZE - 1) / SIZE, units = tiles_v * tiles_t;
     p.x.groups = (count + 31) / 32;
     for (int n = 0;; ++n) {
         const int u = unit_of(n);
         if (n * (int)gridDim.x >= units) break;
         if (u >= units) continue;
         int tv, tt;
-        grouped_tile(u, p.tiles_v, tiles_t, tv, tt);
+        grouped_tile(u, tiles_v, tiles_t, tv, tt);
         typename T::Acc acc;
         T::product(p.W, p.x, tv * T::MG, tt * T::NG, 0, p.W.steps, lds, acc, wave, lane);
-        const int v = tv * TILE + wm * 128, t = tt * TILE + wn * 64;
+        const int v = tv * SIZE + wm * C::WM_ROWS, t = tt * SIZE + wn * C::WN_COLS;
         to_logits(p, acc, v, t, lane);
-        float w[4];
+        float w[BN];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < BN; ++j) {
             const int at = t + 16 * j + (lane & 15);
             const bool live = at < count;
             const int r = live ? g.row_of[at] : 0;
@@ -448,7 +460,7 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
             // The target's place among the lane's values: 16·i + e.
             const int y = (live ? g.targets[r] : -1) - (p.v0 + v + 4 * (lane >> 4));
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < BM; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float x = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * LOG2E);
@@ -457,11 +469,11 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
                 }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < BM / 2; ++i) {
             const int vg = (v >> 5) + i;
             if (vg >= g.steps_v) break;  // wave-uniform
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < BN / 2; ++j) {
                 const int tg = (t >> 5) + j;
                 if (tg >= g.groups_t) break;  // wave-uniform
                 f32x4 c[2][2];
@@ -476,7 +488,7 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
                 for (int q = 0; q < 2; ++q) {
                     f32x4 db = {};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < BN; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) db[e] = fmaf(acc[2 * i + q][j][e], w[j], db[e]);
 #pragma unroll
@@ -484,7 +496,7 @@ __global__ __launch_bounds__(512, 1) void vocab_grad_kernel(Logits p, GradOut g)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) db[e] += __shfl_xor(db[e], o, 64);
                     if ((lane & 15) == 0)
-                        *reinterpret_cast<f32x4*>(g.db_part + (size_t)(tt * 4 + wn) * g.db_pitch + vg * 32 + 16 * q +
+                        *reinterpret_cast<f32x4*>(g.db_part + (size_t)(tt * C::WN + wn) * g.db_pitch + vg * 32 + 16 * q +
                                                   4 * (lane >> 4)) = db;
                 }
             }
@@ -539,22 +551,74 @@ __device__ __forceinline__ Splits plan_splits(const GradProducts& p, int count, 
     return {__builtin_amdgcn_readfirstlane(k % most + 1), __builtin_amdgcn_readfirstlane(k / most + 1)};
 }
 
-// Both products of a piece in one launch.
+// Four values of a row of which `left` more follow.
+__device__ __forceinline__ f32x4 load4(const float* at, int left) {
+    f32x4 v = {};
+    if (left >= 4) {
+        v = *reinterpret_cast<const f32x4_any*>(at);
+    } else if (left > 0) {
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (r < left) v[r] = at[r];
+    }
+    return v;
+}
+__device__ __forceinline__ void store4(float* at, int left, f32x4 v) {
+    if (left >= 4) {
+        *reinterpret_cast<f32x4_any*>(at) = v;
+    } else if (left > 0) {
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+            if (r < left) at[r] = v[r];
+    }
+}
+
+// out[row, h …] (+)= acc·2^e·scale: a lane's values are four neighbours h of the rows row + 16·j. What a row block adds to
+// is read two blocks ahead of its stores.
+template <int BM, int BN>
+__device__ __forceinline__ void put_tile(const f32x4 (&acc)[BM][BN], float* out, int row, int rows, int h, int hidden,
+                                         bool add, int e, float scale) {
+    f32x4 old[3][BN];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < BN; ++j)
+            old[i % 3][j] = add && row + 16 * j < rows
+                                ? load4(out + (size_t)(row + 16 * j) * hidden + h + 16 * i, hidden - h - 16 * i)
+                                : f32x4{};
+    };
+    fetch(0);
+    fetch(1);
+#pragma unroll
+    for (int i = 0; i < BM; ++i) {
+        if (i + 2 < BM) fetch(i + 2);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) {
+            f32x4 v = old[i % 3][j];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += __builtin_amdgcn_ldexpf(acc[i][j][r], e) * scale;
+            if (row + 16 * j < rows) store4(out + (size_t)(row + 16 * j) * hidden + h + 16 * i, hidden - h - 16 * i, v);
+        }
+    }
+}
+
+// Both products of a piece in one launch, transposed: the columns h are the accumulators' rows, four in a row of a lane,
+// so that what is read and written of dW and dx goes 16 bytes at a time.
 template <int PW>
 __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) {
-    typedef Tile<2, 4, 8, 4, 2, 2, true, false> TE;
-    typedef Tile<2, 4, 8, 4, 2, PW, false, true> TX;
+    typedef T256 C;
+    typedef typename C::template Tile<2, 2, false, true> TE;
+    typedef typename C::template Tile<PW, 2, true, false> TX;
     __shared__ __attribute__((aligned(16))) _Float16 lds[TE::LDS_HALVES];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave >> 2, wn = wave & 3;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / C::WN, wn = wave % C::WN;
     const int count = (int)p.words[WORD_COUNT];
     if (count == 0) return;
-    const int tiles_t = (count + TILE - 1) / TILE, steps_v = p.g.steps;
+    const int tiles_t = (count + TILE - 1) / TILE, steps_v = p.g.steps, steps_t = (count + 31) / 32;
     const Splits plan = plan_splits(p, count, gridDim.x, lane);
     const int splits = p.cap_rows ? plan.x : 0, splits_e = plan.e;
     const int tiles_e = p.tiles_v * p.tiles_h, units_e = tiles_e * splits_e;
-    const int units = units_e + tiles_t * p.tiles_h * splits, steps_t = (count + 31) / 32;
+    const int units = units_e + tiles_t * p.tiles_h * splits;
     const int e_wx = -(G_SCALE + pair_scale_exp(p.words[WORD_WX])), e_w = -(G_SCALE + pair_scale_exp(p.words[WORD_W]));
-    p.g.groups = (count + 31) / 32;
+    p.g.groups = steps_t;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         p.words[WORD_SPLITS] = splits;
         p.words[WORD_SPLITS_E] = splits_e;
@@ -567,52 +631,18 @@ __global__ __launch_bounds__(512, 1) void vocab_products_kernel(GradProducts p) 
         if (u < units_e) {
             const int se = u / tiles_e, in = u - se * tiles_e, tv = in / p.tiles_h, th = in - tv * p.tiles_h;
             const int s0 = (int)((long)steps_t * se / splits_e), s1 = (int)((long)steps_t * (se + 1) / splits_e);
-            TE::product(p.g, p.wx, tv * TE::MG, th * TE::NG, s0, s1, lds, acc, wave, lane);
-            float* out = splits_e > 1 ? p.dw_part + (size_t)se * p.vocab * p.hidden : p.dW;
-            const int v = tv * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float old[4][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool in = splits_e == 1 && h + 16 * j < p.hidden && v + 16 * i + r < p.vocab;
-                        old[j][r] = in ? out[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] : 0.0f;
-                    }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (h + 16 * j < p.hidden && v + 16 * i + r < p.vocab)
-                            out[(size_t)(v + 16 * i + r) * p.hidden + h + 16 * j] =
-                                old[j][r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_wx) * p.scale;
-            }
+            TE::product(p.wx, p.g, th * TE::MG, tv * TE::NG, s0, s1, lds, acc, wave, lane);
+            put_tile(acc, splits_e > 1 ? p.dw_part + (size_t)se * p.vocab * p.hidden : p.dW,
+                     tv * TILE + wn * C::WN_COLS + (lane & 15), p.vocab, th * TILE + wm * C::WM_ROWS + 4 * (lane >> 4),
+                     p.hidden, splits_e == 1, e_wx, p.scale);
         } else {
             const int w = u - units_e, per = tiles_t * p.tiles_h, s = w / per, in = w - s * per;
             const int tt = in / p.tiles_h, th = in - tt * p.tiles_h;
             const int s0 = (int)((long)steps_v * s / splits), s1 = (int)((long)steps_v * (s + 1) / splits);
-            TX::product(p.g, p.W, tt * TX::MG, th * TX::NG, s0, s1, lds, acc, wave, lane);
-            const int t = tt * TILE + wm * 128 + 4 * (lane >> 4), h = th * TILE + wn * 64 + (lane & 15);
-            float* out = p.dx_part + (size_t)s * tiles_t * TILE * p.hidden;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float old[4][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        old[j][r] = !p.first && h + 16 * j < p.hidden
-                                        ? out[(size_t)(t + 16 * i + r) * p.hidden + h + 16 * j]
-                                        : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (h + 16 * j < p.hidden)
-                            out[(size_t)(t + 16 * i + r) * p.hidden + h + 16 * j] =
-                                old[j][r] + __builtin_amdgcn_ldexpf(acc[i][j][r], e_w);
-            }
+            TX::product(p.W, p.g, th * TX::MG, tt * TX::NG, s0, s1, lds, acc, wave, lane);
+            put_tile(acc, p.dx_part + (size_t)s * tiles_t * TILE * p.hidden,
+                     tt * TILE + wn * C::WN_COLS + (lane & 15), tiles_t * TILE,
+                     th * TILE + wm * C::WM_ROWS + 4 * (lane >> 4), p.hidden, !p.first, e_w, 1.0f);
         }
     }
 }
@@ -640,6 +670,7 @@ __global__ __launch_bounds__(256) void vocab_dx_kernel(const float* __restrict__
     for (int h = threadIdx.x; h < hidden; h += 256) {
         float s = 0.0f;
         if (j >= 0) {
+#pragma unroll 8
             for (int k = 0; k < splits; ++k) s += part[k * stride + (size_t)j * hidden + h];
             s *= f;
         }
@@ -651,7 +682,7 @@ __global__ __launch_bounds__(256) void vocab_db_kernel(const float* __restrict__
                                                        int vocab, float scale, float* __restrict__ db) {
     const int v = blockIdx.x * 256 + threadIdx.x;
     if (v >= vocab) return;
-    const int n = ((int)words[WORD_COUNT] + TILE - 1) / TILE * 4;
+    const int n = ((int)words[WORD_COUNT] + 63) / 64;
     double s = 0.0;
     for (int k = 0; k < n; ++k) s += part[(size_t)k * pitch + v];
     db[v] += (float)(s * (double)scale * (1.0 / (1 << G_SCALE)));
@@ -728,7 +759,22 @@ int piece_rows(const laya_ctx* ctx, int vocab, size_t each, size_t fixed) {
     return (int)std::min<long>(pad_tile((vocab + pieces - 1) / pieces), pad_tile(vocab));
 }
 
-int workgroups(const laya_ctx* ctx) { return std::max(8, ctx->cu_count / 8 * 8); }
+template <class C>
+int workgroups(const laya_ctx* ctx) { return std::max(8, ctx->cu_count / 8 * 8) * C::PER_CU; }
+
+// f(the tile of a launch of `rows` x `vocab` logits). A round of 256 tiles over the chip takes about as long as three units a
+// CU of 128 tiles (57 us and 19 us over 768 columns), which fill the last round better, two to a CU hide each other's ends,
+// and a small problem gets on more CUs: 600 rows x 50368 stats 131 us on 128 and 173 on 256, 400 rows 119 and 115, 4915
+// rows 976 and 925; 487 x 7905 34 and 57.
+template <class F> void with_tile(laya_ctx* ctx, long rows, long vocab, F&& f) {
+    const long G = workgroups<T256>(ctx), large = pad_tile(rows) / 256 * (pad_tile(vocab) / 256),
+               small = (rows + 127) / 128 * ((vocab + 127) / 128);
+    const double by_small = std::max(0.6, (double)small / (3.0 * G) + 0.15);
+    if (by_small < (double)((large + G - 1) / G))
+        f(T128());
+    else
+        f(T256());
+}
 
 }  // namespace
 
@@ -762,9 +808,9 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
     }
     if (vocab_few_rows(a)) return vocab_few_fwd(ctx, a, row_loss, lse, loss, bad_count);
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
-    const int tiles = (a.vocab + TILE - 1) / TILE;
+    const int most_tiles = (a.vocab + 127) / 128;
     const int piece = piece_rows(ctx, a.vocab, (size_t)steps_of(a.hidden) * 64 * planes + 8,
-                                 2 * halves(a.rows, a.hidden, 2) + 8 * ((size_t)tiles + 1) * pitch);
+                                 2 * halves(a.rows, a.hidden, 2) + 8 * ((size_t)most_tiles + 1) * pitch);
     unsigned* words;
     int *row_of, *ex, *ew;
     float* padded;
@@ -778,22 +824,27 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
         ws.take(padded, piece);
         ws.take(xp, halves(a.rows, a.hidden, 2));
         ws.take(wp, halves(piece, a.hidden, planes));
-        ws.take(part, (size_t)tiles * pitch);
+        ws.take(part, (size_t)most_tiles * pitch);
     });
     LAYA_LAUNCH(label_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, a.targets, a.rows, a.vocab, row_of,
                 (int*)nullptr, words, bad_count, row_loss, lse);
     check_launch("label_rows_kernel");
     pack_states(ctx, a, row_of, words, ex, xp, false);
+    int tiles = 0;
     for (int v0 = 0; v0 < a.vocab; v0 += piece) {
         const int n = std::min(piece, a.vocab - v0);
         pack_table(ctx, a, v0, n, nullptr, ew, padded, wp);
-        Logits p{{wp, steps_of(a.hidden), groups_of(n)}, {xp, steps_of(a.hidden), 0}, ew, ex, padded, words, v0, n,
-                 (n + TILE - 1) / TILE};
+        Logits p{{wp, steps_of(a.hidden), groups_of(n)}, {xp, steps_of(a.hidden), 0}, ew, ex, padded, words, v0, n};
         ProfileScope scope(ctx, "vocab_stats", 2.0 * a.rows * a.hidden * n, 0.0);
-        if (a.W16)
-            LAYA_LAUNCH(vocab_stats_kernel<1>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, p, part, pitch);
-        else
-            LAYA_LAUNCH(vocab_stats_kernel<2>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, p, part, pitch);
+        with_tile(ctx, a.rows, std::min(piece, a.vocab), [&](auto c) {
+            typedef decltype(c) C;
+            const dim3 grid(workgroups<C>(ctx)), block(C::THREADS);
+            if (a.W16)
+                LAYA_LAUNCH((vocab_stats_kernel<C, 1>), grid, block, 0, ctx->stream, p, part, pitch);
+            else
+                LAYA_LAUNCH((vocab_stats_kernel<C, 2>), grid, block, 0, ctx->stream, p, part, pitch);
+            tiles = (a.vocab + C::SIZE - 1) / C::SIZE;
+        });
         check_launch("vocab_stats_kernel");
     }
     vocab_merge(ctx, a, part, pitch, tiles, words, row_of, row_loss, lse, loss);
@@ -813,7 +864,7 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
     // dW's partial sums: a table of few tiles, whole in one piece, takes as many splits as fill the chip twice.
     const int tiles_e = dW && piece >= a.vocab ? (a.vocab + TILE - 1) / TILE * tiles_h : 0;
     const int most_e =
-        tiles_e && !ctx->cap ? std::max(1, std::min({MAX_SPLITS, 2 * workgroups(ctx) / tiles_e, steps_t / 8})) : 1;
+        tiles_e && !ctx->cap ? std::max(1, std::min({MAX_SPLITS, 2 * workgroups<T256>(ctx) / tiles_e, steps_t / 8})) : 1;
     unsigned* words;
     int *row_of, *place, *ex, *ew;
     float *padded, *part, *db_part, *dw_part;
@@ -851,19 +902,22 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
             units_e = dW ? tiles_v * tiles_h : 0;
         }
         pack_table(ctx, a, v0, n, words + WORD_W, ew, padded, wp);
-        Logits p{{wp, steps_h, groups_of(n)}, {xp, steps_h, 0}, ew, ex, padded, words, v0, n, tiles_v};
+        Logits p{{wp, steps_h, groups_of(n)}, {xp, steps_h, 0}, ew, ex, padded, words, v0, n};
         GradOut g{row_of, a.targets, lse, a.row_weights, gp, steps_of(n), steps_t, db_part, piece};
         {
             ProfileScope scope(ctx, "vocab_grad", 2.0 * a.rows * a.hidden * n, 0.0);
-            const dim3 grid(workgroups(ctx)), block(512);
-            if (a.W16 && db)
-                LAYA_LAUNCH((vocab_grad_kernel<1, true>), grid, block, 0, ctx->stream, p, g);
-            else if (a.W16)
-                LAYA_LAUNCH((vocab_grad_kernel<1, false>), grid, block, 0, ctx->stream, p, g);
-            else if (db)
-                LAYA_LAUNCH((vocab_grad_kernel<2, true>), grid, block, 0, ctx->stream, p, g);
-            else
-                LAYA_LAUNCH((vocab_grad_kernel<2, false>), grid, block, 0, ctx->stream, p, g);
+            with_tile(ctx, a.rows, std::min(piece, a.vocab), [&](auto c) {
+                typedef decltype(c) C;
+                const dim3 grid(workgroups<C>(ctx)), block(C::THREADS);
+                if (a.W16 && db)
+                    LAYA_LAUNCH((vocab_grad_kernel<C, 1, true>), grid, block, 0, ctx->stream, p, g);
+                else if (a.W16)
+                    LAYA_LAUNCH((vocab_grad_kernel<C, 1, false>), grid, block, 0, ctx->stream, p, g);
+                else if (db)
+                    LAYA_LAUNCH((vocab_grad_kernel<C, 2, true>), grid, block, 0, ctx->stream, p, g);
+                else
+                    LAYA_LAUNCH((vocab_grad_kernel<C, 2, false>), grid, block, 0, ctx->stream, p, g);
+            });
             check_launch("vocab_grad_kernel");
         }
         GradProducts q{};
@@ -886,10 +940,11 @@ void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx
         q.most_e = most_e;
         if (dx || dW) {
             ProfileScope scope(ctx, "vocab_products", ((dx ? 2.0 : 0.0) + (dW ? 2.0 : 0.0)) * a.rows * a.hidden * n, 0.0);
+            const dim3 grid(workgroups<T256>(ctx)), block(512);
             if (a.W16)
-                LAYA_LAUNCH(vocab_products_kernel<1>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, q);
+                LAYA_LAUNCH(vocab_products_kernel<1>, grid, block, 0, ctx->stream, q);
             else
-                LAYA_LAUNCH(vocab_products_kernel<2>, dim3(workgroups(ctx)), dim3(512), 0, ctx->stream, q);
+                LAYA_LAUNCH(vocab_products_kernel<2>, grid, block, 0, ctx->stream, q);
             check_launch("vocab_products_kernel");
         }
         if (most_e > 1) {
