@@ -286,7 +286,8 @@ int laya_adamw(laya_ctx* ctx, float* params, float* grads, float* m, float* v, i
 int laya_orthogonalize(laya_ctx* ctx, const float* x, int count, int rows, int cols, int steps, float* out);
 
 /* Matrices inside a flat arena, for laya_muon: matrix i is [rows[i], cols[i]] from element offset[i] (host arrays; no two
- * overlap), its update scaled by multiplier[i] (NULL: 1). They may be of any shapes; equal ones share launches. */
+ * overlap), its update scaled by multiplier[i] (NULL: 1). They may be of any shapes up to 2^20 a side and 2^31 − 2^16
+ * elements (as laya_orthogonalize's); equal ones share launches. */
 int laya_matrices_create(laya_ctx* ctx, const size_t* offset, const int* rows, const int* cols, const float* multiplier,
                          int n, laya_matrices** out);
 int laya_matrices_destroy(laya_ctx* ctx, laya_matrices* matrices);

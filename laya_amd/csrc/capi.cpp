@@ -976,7 +976,8 @@ int laya_adamw(laya_ctx* ctx, float* params, float* grads, float* m, float* v, i
 }
 
 static void check_matrix(const char* what, long rows, long cols) {
-    LAYA_REQUIRE(rows > 0 && cols > 0 && rows <= 1 << 20 && cols <= 1 << 20 && rows * cols < 1ll << 31,
+    // Under 2^31 elements by more than a chunk of the norm's sums, so that their ends fit an int.
+    LAYA_REQUIRE(rows > 0 && cols > 0 && rows <= 1 << 20 && cols <= 1 << 20 && rows * cols <= (1ll << 31) - (1 << 16),
                  std::string(what) + ": a matrix of " + std::to_string(rows) + " x " + std::to_string(cols));
 }
 
@@ -1015,6 +1016,7 @@ int laya_matrices_create(laya_ctx* ctx, const size_t* offset, const int* rows, c
         });
         DeviceScope device(ctx);
         auto* m = new laya_matrices();
+        m->device = ctx->device;
         try {
             for (int i : order) {
                 if (m->runs.empty() || m->runs.back().rows != rows[i] || m->runs.back().cols != cols[i])
@@ -1025,11 +1027,12 @@ int laya_matrices_create(laya_ctx* ctx, const size_t* offset, const int* rows, c
             }
             m->d_offsets = static_cast<size_t*>(ctx->alloc(sizeof(size_t) * std::max(n, 1)));
             m->d_multipliers = static_cast<float*>(ctx->alloc(sizeof(float) * std::max(n, 1)));
-            if (n) {  // the host vectors live as long as the handle, whose end waits for the stream
+            if (n) {  // waited for: the handle may be used on another context's stream
                 LAYA_HIP(hipMemcpyAsync(m->d_offsets, m->offsets.data(), sizeof(size_t) * n, hipMemcpyHostToDevice,
                                         ctx->stream));
                 LAYA_HIP(hipMemcpyAsync(m->d_multipliers, m->multipliers.data(), sizeof(float) * n,
                                         hipMemcpyHostToDevice, ctx->stream));
+                LAYA_HIP(hipStreamSynchronize(ctx->stream));
             }
         } catch (...) {
             if (m->d_offsets) ctx->release(m->d_offsets);
@@ -1057,6 +1060,7 @@ int laya_muon(laya_ctx* ctx, const laya_matrices* matrices, float* params, float
     return guarded([&] {
         require_ctx(ctx);
         LAYA_REQUIRE(matrices, "muon: null matrices");
+        LAYA_REQUIRE(matrices->device == ctx->device, "muon: matrices of another device");
         LAYA_REQUIRE(matrices->offsets.empty() || (params && grads && momentum), "muon: null arena");
         LAYA_REQUIRE(std::isfinite(lr) && std::isfinite(weight_decay) && mu >= 0 && mu < 1,
                      "muon: lr and weight_decay finite, mu in [0, 1)");

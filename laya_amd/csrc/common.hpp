@@ -151,6 +151,7 @@ struct laya_matrices {
     std::vector<Run> runs;
     std::vector<size_t> offsets;
     std::vector<float> multipliers;
+    int device = 0;
     size_t* d_offsets = nullptr;
     float* d_multipliers = nullptr;
 };

@@ -270,6 +270,40 @@ def test_refusals(ctx):
         ops.muon(m, a, b, DeviceArray(ctx, (20,)), 0.1)
 
 
+@pytest.mark.parametrize("rows,cols", [(1048575, 2048), (2048, 1048575), (46341, 46341), (1 << 20, 1 << 20)])
+def test_sizes_past_an_int_are_refused(ctx, rows, cols):
+    """2^31 elements, and the last few below it, where the ends of the norm's chunks would not fit an int."""
+    from laya_amd import ops
+    from laya_amd._native import ERR_ARGUMENT, LayaArgumentError, lib
+    from laya_amd.device import DeviceArray
+    a = DeviceArray(ctx, (64,))
+    assert lib().laya_orthogonalize(ctx.handle, a.ptr, 1, rows, cols, 5, a.ptr) == ERR_ARGUMENT
+    with pytest.raises(LayaArgumentError, match=f"{rows} x {cols}"):
+        ops.MuonMatrices(ctx, [0], [rows], [cols])
+
+
+def test_matrices_of_another_context(ctx):
+    """The tables are on the device when the call returns: another context's stream may read them at once."""
+    from laya_amd import ops
+    from laya_amd.device import Context, DeviceArray
+    r = np.random.default_rng(4)
+    p, g = (r.standard_normal(24 * 40).astype(np.float32) for _ in range(2))
+    out = []
+    other = Context(ctx.device)
+    try:
+        for run in (ctx, other):
+            P, G, M = (DeviceArray.from_numpy(run, v) for v in (p, g, np.zeros_like(p)))
+            run.sync()
+            m = ops.MuonMatrices(ctx, [0], [24], [40])
+            m.ctx = run
+            ops.muon(m, P, G, M, 0.1)
+            out.append(P.numpy())
+            m.ctx = ctx
+    finally:
+        other.close()
+    np.testing.assert_array_equal(out[0], out[1])
+
+
 def test_no_matrices_to_move(ctx):
     from laya_amd import ops
     from laya_amd.device import DeviceArray
