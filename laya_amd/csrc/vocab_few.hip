@@ -227,8 +227,9 @@ struct FewLogits {
 
 // Blocks of 16 rows of W a wave takes: with many rows of x it is their reads from LDS that two blocks share.
 constexpr int wave_blocks(int nb) { return nb >= 8 ? 2 : 1; }
-// Steps of a ring: what is under way of W waits in registers.
-constexpr int ring_of(int nb) { return nb >= 12 ? 3 : 4; }
+// Steps of a ring: what is under way of W waits in registers. At 16 blocks the sums leave room for two (256 rows x 768 x
+// 50368 both ways 527 us; with three, which spill more, 556).
+constexpr int ring_of(int nb) { return nb >= 16 ? 2 : nb >= 12 ? 3 : 4; }
 
 // A workgroup is as many waves, WAVES at least, as spread the table's blocks of 16 rows evenly over the CUs.
 template <int NB, typename TW, bool GRAD, int WAVES>
@@ -331,7 +332,8 @@ __global__ __launch_bounds__(1024 / wave_blocks(NB), 1) void few_logits_kernel(F
     for (int s = 0; s < steps; s += RING) {
         step(s, std::integral_constant<int, 0>());
         if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
-        if (s + 2 < steps) step(s + 2, std::integral_constant<int, 2>());
+        if constexpr (RING > 2)
+            if (s + 2 < steps) step(s + 2, std::integral_constant<int, 2>());
         if constexpr (RING == 4)
             if (s + 3 < steps) step(s + 3, std::integral_constant<int, 3>());
     }
