@@ -11,6 +11,13 @@
 // Scales of the two-piece products (powers of two, so that scaling is exact): x by row, G by 2^14, w_t·x_t as a whole. W
 // by row in the forward; as a whole in the backward, where one packed W serves the logits (over its columns) and dx
 // (over its rows), as one packed G serves dx and dW.
+//
+// The matrix cores bound it, at the clock that their power leaves: a large fp16 library product of random values reaches
+// 1.46 PFLOP/s on this card, 487 TFLOP/s of three products each. 4915 labelled rows x 768 x 50368: statistics 0.95 ms (399
+// TFLOP/s of fp32 products), G 1.05 ms (362; it also writes 1 GB of pieces), the two gradient products 1.89 ms (403). What
+// remains is copies: packing W 64 us (310 MB, 4.8 TB/s) in either direction, its largest magnitude 41 us (155 MB). Packing
+// first pays because a tile's operands are read by every tile of their row and column: pieces are copied to LDS as they
+// are, without a split in the product's loop.
 #include "elementwise.hpp"
 #include "packed.hpp"
 #include "vocab.hpp"
