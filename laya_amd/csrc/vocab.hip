@@ -261,6 +261,10 @@ __global__ __launch_bounds__(256) void pack_weighted_kernel(const float* __restr
 
 // ------------------------------------------------------------------------------- logits and what they become
 
+struct Targets {
+    const int *row_of, *targets;
+    float* z_target;           // [labelled row]
+};
 struct Logits {
     Operand W, x;              // W's piece: rows v; x: rows t
     const int *ew, *ex;        // their rows' scale exponents
@@ -296,9 +300,11 @@ __device__ __forceinline__ void to_logits(const Logits& p, f32x4 (&acc)[BM][BN],
     }
 }
 
-// Each tile's maximum and Σ exp(z − maximum) for every row (token): part[tile_v][t].
+// Each tile's maximum and Σ exp(z − maximum) for every row (token): part[tile_v][t]. The target's logit, where the tile has
+// it, goes to z_target[t]: the one that is in the sum, so that what its product is off by cancels in a small loss.
 template <class C, int PW>
-__global__ __launch_bounds__(C::THREADS, C::PER_CU) void vocab_stats_kernel(Logits p, float2* __restrict__ part, int pitch) {
+__global__ __launch_bounds__(C::THREADS, C::PER_CU) void vocab_stats_kernel(Logits p, Targets y,
+                                                                                        float2* __restrict__ part, int pitch) {
     typedef typename C::template Tile<PW, 2> T;
     constexpr int SIZE = C::SIZE, BM = C::BM, BN = C::BN;
     __shared__ __attribute__((aligned(16))) _Float16 lds[T::LDS_HALVES];
@@ -314,7 +320,19 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU) void vocab_stats_kernel(Logi
         grouped_tile(u, tiles_v, tiles_t, tv, tt);
         typename T::Acc acc;
         T::product(p.W, p.x, tv * T::MG, tt * T::NG, 0, p.W.steps, lds, acc, wave, lane);
-        to_logits(p, acc, tv * SIZE + wm * C::WM_ROWS, tt * SIZE + wn * C::WN_COLS, lane);
+        const int v = tv * SIZE + wm * C::WM_ROWS, t = tt * SIZE + wn * C::WN_COLS;
+        to_logits(p, acc, v, t, lane);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) {
+            const int at = t + 16 * j + (lane & 15);
+            const int where = (at < count ? y.targets[y.row_of[at]] : -1) - (p.v0 + v + 4 * (lane >> 4));
+            if (!__any(where >= 0 && where < 16 * BM)) continue;
+#pragma unroll
+            for (int i = 0; i < BM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (where == 16 * i + r) y.z_target[at] = acc[i][j][r];
+        }
         float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
         for (int j = 0; j < BN; ++j) {
@@ -374,39 +392,17 @@ __global__ __launch_bounds__(1024) void vocab_total_kernel(const int* row_of, co
     total_loss<1024>(row_of, (int)words[WORD_COUNT], row_loss, weights, scale, loss);
 }
 
-// One wave a labelled row: the tiles' statistics merged, and the target's logit from W's row itself. With `loss` the last
-// workgroup to end sums the rows' weighted losses.
-template <typename TW>
+// One wave a labelled row: the tiles' statistics merged, less the target's logit. With `loss` the last workgroup to end sums
+// the rows' weighted losses.
 __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restrict__ part, int pitch, int tiles,
                                                           unsigned* words, const int* __restrict__ row_of,
-                                                          const int* __restrict__ targets, const float* __restrict__ x,
-                                                          const TW* __restrict__ W, const float* __restrict__ bias,
-                                                          int hidden, float* row_loss, float* __restrict__ lse,
-                                                          const float* __restrict__ weights, float scale, float* loss) {
+                                                          const float* __restrict__ z_target, float* row_loss,
+                                                          float* __restrict__ lse, const float* __restrict__ weights,
+                                                          float scale, float* loss) {
     const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, count = (int)words[WORD_COUNT];
     if (j < count) {
-        const int r = row_of[j], y = targets[r];
-        // The target's row first: its loads are under way while the tiles' arrive.
-        const float* xr = x + (size_t)r * hidden;
-        const TW* wr = W + (size_t)y * hidden;
-        double z = 0.0, z1 = 0.0;
-        int k0 = lane;
-#pragma unroll 2
-        for (; k0 + 448 < hidden; k0 += 512) {
-            float xv[8], wv[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                xv[q] = xr[k0 + 64 * q];
-                wv[q] = (float)wr[k0 + 64 * q];
-            }
-#pragma unroll
-            for (int q = 0; q < 8; q += 2) {
-                z += (double)xv[q] * wv[q];
-                z1 += (double)xv[q + 1] * wv[q + 1];
-            }
-        }
-#pragma unroll 4
-        for (; k0 < hidden; k0 += 64) z += (double)xr[k0] * (double)(float)wr[k0];
+        const int r = row_of[j];
+        const float z = z_target[j];
         // Each lane's tiles, four at a time: the maximum and the sum so far.
         float m = -__builtin_inff(), s = 0.0f;
         for (int k = lane; k < tiles; k += 256) {
@@ -426,11 +422,10 @@ __global__ __launch_bounds__(256) void vocab_merge_kernel(const float2* __restri
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
         const float at = top == -__builtin_inff() ? 0.0f : top;
         const double sum = wave_sum_d((double)(s * __builtin_amdgcn_exp2f((m - at) * LOG2E)));
-        z = wave_sum_d(z + z1);
         if (lane == 0) {
-            const double l = (double)top + log(sum);
-            lse[r] = (float)l;
-            __hip_atomic_store(row_loss + r, (float)(l - (z + (bias ? (double)bias[y] : 0.0))), __ATOMIC_RELAXED,
+            const double l = log(sum);
+            lse[r] = (float)((double)top + l);
+            __hip_atomic_store(row_loss + r, (float)(((double)top - (double)z) + l), __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
         }
     }
@@ -805,19 +800,12 @@ template <class F> void with_tile(laya_ctx* ctx, long rows, long vocab, F&& f) {
 }  // namespace
 
 void vocab_merge(laya_ctx* ctx, const VocabArgs& a, const float2* part, int pitch, int tiles, unsigned* words,
-                 const int* row_of, float* row_loss, float* lse, float* loss) {
+                 const int* row_of, const float* z_target, float* row_loss, float* lse, float* loss) {
     // The total by the last workgroup saves a launch (4 of 52 µs at 19 rows), but its fences cost 0.07 µs a workgroup, one
     // after another: 250 µs at 13871 rows, where a launch of its own takes 6.
     const bool own = a.rows > VOCAB_FEW;
-    const dim3 grid((a.rows + 3) / 4);
-    if (a.W16)
-        LAYA_LAUNCH(vocab_merge_kernel<__bf16>, grid, dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
-                    a.targets, a.x, a.W16, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale,
-                    own ? nullptr : loss);
-    else
-        LAYA_LAUNCH(vocab_merge_kernel<float>, grid, dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
-                    a.targets, a.x, a.W, a.bias, a.hidden, row_loss, lse, a.row_weights, a.scale,
-                    own ? nullptr : loss);
+    LAYA_LAUNCH(vocab_merge_kernel, dim3((a.rows + 3) / 4), dim3(256), 0, ctx->stream, part, pitch, tiles, words, row_of,
+                z_target, row_loss, lse, a.row_weights, a.scale, own ? nullptr : loss);
     check_launch("vocab_merge_kernel");
     if (loss && own) {
         LAYA_LAUNCH(vocab_total_kernel, dim3(1), dim3(1024), 0, ctx->stream, row_of, words, row_loss, a.row_weights,
@@ -836,10 +824,10 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
     const int planes = a.W16 ? 1 : 2, pitch = (int)pad_tile(a.rows);
     const int most_tiles = (a.vocab + 127) / 128;
     const int piece = piece_rows(ctx, a.vocab, (size_t)steps_of(a.hidden) * 64 * planes + 8,
-                                 2 * halves(a.rows, a.hidden, 2) + 8 * ((size_t)most_tiles + 1) * pitch);
+                                 2 * halves(a.rows, a.hidden, 2) + 8 * ((size_t)most_tiles + 2) * pitch);
     unsigned* words;
     int *row_of, *ex, *ew;
-    float* padded;
+    float *padded, *z_target;
     _Float16 *xp, *wp;
     float2* part;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
@@ -848,6 +836,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
         ws.take(ex, pitch);
         ws.take(ew, piece);
         ws.take(padded, piece);
+        ws.take(z_target, a.rows);
         ws.take(xp, halves(a.rows, a.hidden, 2));
         ws.take(wp, halves(piece, a.hidden, planes));
         ws.take(part, (size_t)most_tiles * pitch);
@@ -856,6 +845,7 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
                 (int*)nullptr, words, bad_count, row_loss, lse);
     check_launch("label_rows_kernel");
     pack_states(ctx, a, row_of, words, ex, xp, false);
+    const Targets y{row_of, a.targets, z_target};
     int tiles = 0;
     for (int v0 = 0; v0 < a.vocab; v0 += piece) {
         const int n = std::min(piece, a.vocab - v0);
@@ -866,14 +856,14 @@ void vocab_ce_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse
             typedef decltype(c) C;
             const dim3 grid(workgroups<C>(ctx)), block(C::THREADS);
             if (a.W16)
-                LAYA_LAUNCH((vocab_stats_kernel<C, 1>), grid, block, 0, ctx->stream, p, part, pitch);
+                LAYA_LAUNCH((vocab_stats_kernel<C, 1>), grid, block, 0, ctx->stream, p, y, part, pitch);
             else
-                LAYA_LAUNCH((vocab_stats_kernel<C, 2>), grid, block, 0, ctx->stream, p, part, pitch);
+                LAYA_LAUNCH((vocab_stats_kernel<C, 2>), grid, block, 0, ctx->stream, p, y, part, pitch);
             tiles = (a.vocab + C::SIZE - 1) / C::SIZE;
         });
         check_launch("vocab_stats_kernel");
     }
-    vocab_merge(ctx, a, part, pitch, tiles, words, row_of, row_loss, lse, loss);
+    vocab_merge(ctx, a, part, pitch, tiles, words, row_of, z_target, row_loss, lse, loss);
 }
 
 void vocab_ce_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {

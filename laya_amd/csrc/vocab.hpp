@@ -44,9 +44,9 @@ __device__ __forceinline__ void load8(const T* row, int c, int K, float (&v)[8])
     }
 }
 
-// The tiles' statistics part[tile][pitch] into row_loss, lse and the weighted total.
+// The tiles' statistics part[tile][pitch] and the targets' logits into row_loss, lse and the weighted total.
 void vocab_merge(laya_ctx* ctx, const VocabArgs& a, const float2* part, int pitch, int tiles, unsigned* words,
-                 const int* row_of, float* row_loss, float* lse, float* loss);
+                 const int* row_of, const float* z_target, float* row_loss, float* lse, float* loss);
 bool vocab_few_rows(const VocabArgs& a);
 void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* lse, float* loss, int* bad_count);
 void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db);

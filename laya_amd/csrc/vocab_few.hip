@@ -218,11 +218,12 @@ struct FewLogits {
     const int* exps;
     unsigned* words;
     int hidden, vocab, steps, blocks_v;  // blocks_v: blocks of 16 rows of W, an even number
+    const int *row_of, *targets;
     // Statistics:
     float2* part;            // [workgroup][pitch]
     int pitch;
+    float* z_target;         // [labelled row]: the target's logit as it is in the sum
     // G:
-    const int *row_of, *targets;
     const float *lse, *weights;
     _Float16* g_rows;        // [step of 32 v][block of t][2][FRAG]: rows t over v
     _Float16* g_cols;        // [block of 16 v][step of 32 t][2][FRAG]: rows v over t
@@ -355,6 +356,19 @@ __global__ __launch_bounds__(1024 / wave_blocks(NB), 1) void few_logits_kernel(F
                 acc[i][j][r] = __builtin_amdgcn_ldexpf(acc[i][j][r], -(e + p.exps[16 * j + (lane & 15)])) + b;
         }
     if constexpr (!GRAD) {
+        if (v0 < p.blocks_v * 16) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int t = 16 * j + (lane & 15);
+                const int where = (t < count ? p.targets[p.row_of[t]] : -1) - (v0 + 4 * (lane >> 4));
+                if (!__any(where >= 0 && where < 16 * VB)) continue;
+#pragma unroll
+                for (int i = 0; i < VB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (where == 16 * i + r) p.z_target[t] = acc[i][j][r];
+            }
+        }
         float2* red = reinterpret_cast<float2*>(lds);  // [wave][16·NB]
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
@@ -742,12 +756,14 @@ void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* ls
     _Float16* x_rows;
     int* exps;
     float2* part;
+    float* z_target;
     carve(ctx, VOCAB_SLOT, [&](Carve& ws) {
         ws.take(words, WORDS);
         ws.take(row_of, a.rows);
         ws.take(exps, 16 * nb);
         ws.take(x_rows, (size_t)steps * nb * BLOCK);
         ws.take(part, (size_t)tiles * pitch);
+        ws.take(z_target, pitch);
     });
     const Prepare prep{a.x, a.row_weights, a.targets, a.rows, a.hidden, a.vocab, nb, x_rows, nullptr, exps,
                        row_of, nullptr, bad_count, words, row_loss, lse};
@@ -762,10 +778,13 @@ void vocab_few_fwd(laya_ctx* ctx, const VocabArgs& a, float* row_loss, float* ls
     p.vocab = a.vocab;
     p.steps = steps;
     p.blocks_v = blocks_v;
+    p.row_of = row_of;
+    p.targets = a.targets;
     p.part = part;
+    p.z_target = z_target;
     p.pitch = pitch;
     launch_logits<false>(ctx, a, p, nb);
-    vocab_merge(ctx, a, part, pitch, tiles, words, row_of, row_loss, lse, loss);
+    vocab_merge(ctx, a, part, pitch, tiles, words, row_of, z_target, row_loss, lse, loss);
 }
 
 void vocab_few_bwd(laya_ctx* ctx, const VocabArgs& a, const float* lse, float* dx, float* dW, float* db) {

@@ -69,7 +69,8 @@ def _exact(p):
     dG = p_abs * (dz + dlse[:, None] + 4 * U * (2 + np.abs(finite_z - lse[:, None]))) + 4 * U * np.abs(G / np.maximum(
         w * p["scale"], 1e-300)[:, None]) + 2.0 ** -38
     dG *= w[:, None] * p["scale"]
-    tol = {"row_loss": dlse + 4 * U * (np.abs(lse) + np.abs(np.where(np.isfinite(z[n, at]), z[n, at], 0))),
+    # row_loss = lse − z_y of the logit that the sum holds: |δ_lse| + |δ_z_y| at most, and the two roundings.
+    tol = {"row_loss": dlse + dz[n, at] + 4 * U * (np.abs(lse) + np.abs(np.where(np.isfinite(z[n, at]), z[n, at], 0))),
            "lse": dlse, "dx": dG @ np.abs(W) + product(G, W, vocab) + 4 * U * np.abs(out["dx"]),
            "dW": dG.T @ np.abs(x) + product(G.T, x, rows) + 4 * U * np.abs(out["dW"]),
            "db": dG.sum(0) + (2 + rows) * U * np.abs(G).sum(0) + 4 * U * np.abs(out["db"])}
@@ -273,6 +274,30 @@ def test_zero_weight_and_hidden_rows(ctx):
         p["W"][:] = 0
         want, tol = _exact(p)
         _check(_run(ctx, p), want, tol)
+
+
+@pytest.mark.parametrize("rows", [30, 150, 250, 330, 1400])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_small_losses_of_large_logits(ctx, rows, bf16):
+    """A target ahead of the next entry by ten, with logits of 200: loss = log(1 + s), s = Σ_{v ≠ y} exp(z_v − z_y). The
+    target's logit is in the sum as it is subtracted, so its own error e moves the loss by e·s / (1 + s), as the others'
+    do: 2·e·s in all. Beside that the sum is near one and is off by a few roundings: of up to 32 values a lane, 6 exchanges
+    and as many merges, 64·U."""
+    p = _problem(rows, 256, 600, bias=False)
+    p["W"][1::2] = np.float32(0.95) * p["W"][::2]
+    if bf16:
+        p["W"], p["bits"] = _bf16(p["W"])
+    p["t"] = (p["t"] // 2 * 2).astype(np.int32)
+    target = p["W"][p["t"]].astype(np.float64)
+    p["x"] = (200 * target / (target ** 2).sum(1, keepdims=True)).astype(np.float32)
+    W, x = p["W"].astype(np.float64), p["x"].astype(np.float64)
+    z, off = x @ W.T, (12 * U + 256 * U) * (np.abs(x) @ np.abs(W).T)
+    n = np.arange(rows)
+    d = z - z[n, p["t"]][:, None]
+    d[n, p["t"]] = -np.inf
+    s = np.exp(d).sum(1)
+    got = _run(ctx, p, backward=False)
+    assert (np.abs(got["row_loss"] - np.log1p(s)) <= 2 * s * (off + 2 * U * np.abs(z)).max(1) + 64 * U).all()
 
 
 @pytest.mark.parametrize("rows", [77, 600])
