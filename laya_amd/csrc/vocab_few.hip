@@ -12,7 +12,7 @@
 // Fragments are 16 rows x 32 k of v_mfma_f32_16x16x32_f16, [k / 8][row][8 k], the two planes one after another.
 //
 // A large copy runs at 5.0 TB/s on this card. 19 rows x 768 x 50368: logits 33.7 us (W's 155 MB at 4.6 TB/s); the merge and
-// the preparation are 8 and 6 us of latency. 77 rows both ways: logits 43 and 50 us, dx 47 us (3.3 TB/s: a lane's loads go
+// the preparation are 6 us of latency each. 77 rows both ways: logits 43 and 50 us, dx 47 us (3.3 TB/s: a lane's loads go
 // down W's columns, eight bytes a row), dW 78 us (310 MB read and written, 4.0 TB/s). With more rows the splits and x's
 // reads from LDS come to weigh as much: 192 rows 0.35 ms both ways, 256 rows 0.53 ms.
 #include "elementwise.hpp"
