@@ -56,15 +56,16 @@ __device__ __forceinline__ void split_value(float v, _Float16& hi, _Float16& lo)
 template <int KB>
 __device__ __forceinline__ void copy_to_lds(const _Float16* from, unsigned to) {
     static_assert(KB == 2 || KB == 4, "a row group's step");
+    constexpr int KIB = 1024;
     if constexpr (KB == 4)
         asm volatile(
             "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-            "global_load_lds_dwordx4 %1, off offset:1024\n\tglobal_load_lds_dwordx4 %1, off offset:2048\n\t"
-            "global_load_lds_dwordx4 %1, off offset:3072" ::"s"(to), "v"(from) : "memory");
+            "global_load_lds_dwordx4 %1, off offset:%2\n\tglobal_load_lds_dwordx4 %1, off offset:%3\n\t"
+            "global_load_lds_dwordx4 %1, off offset:%4" ::"s"(to), "v"(from), "n"(KIB), "n"(2 * KIB), "n"(3 * KIB) : "memory");
     else
         asm volatile(
             "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-            "global_load_lds_dwordx4 %1, off offset:1024" ::"s"(to), "v"(from) : "memory");
+            "global_load_lds_dwordx4 %1, off offset:%2" ::"s"(to), "v"(from), "n"(KIB) : "memory");
 }
 // Waits for all but the wave's last N copies (and its other memory accesses before them), then for the whole workgroup:
 // what every wave copied before its last N is in LDS, and every wave's reads before this point are done.
