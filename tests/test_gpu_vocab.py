@@ -367,6 +367,53 @@ def test_unaligned_table_and_states(ctx):
                 "db": b.gradient.numpy()}, want, tol)
 
 
+@pytest.mark.parametrize("rows", [5, 300])
+def test_a_table_of_more_than_2_31_values(ctx, rows):
+    """1,100,000 x 2048: zeros but for the last 64 rows, which lie past an int's range of elements. A row's logits are then
+    64 numbers and zeros, whose exponentials, ones, add without error."""
+    from laya_amd import ops
+    from laya_amd.device import DeviceArray
+    vocab, hidden, last = 1_100_000, 2048, 64
+    r = np.random.default_rng(rows)
+    x = r.standard_normal((rows, hidden)).astype(np.float32)
+    w = (r.standard_normal((last, hidden)) * 4 / np.sqrt(hidden)).astype(np.float32)
+    t = (vocab - 1 - r.integers(0, last, rows)).astype(np.int32)
+    W, dW = DeviceArray(ctx, (vocab, hidden)), DeviceArray(ctx, (vocab, hidden))
+    try:
+        W.fill(0.0)
+        dW.fill(0.0)
+        part = lambda a, v: DeviceArray.borrow(ctx, a.ptr + 4 * v * hidden, (last, hidden), owner=a)  # noqa: E731
+        part(W, vocab - last).upload(w)
+        P = ops.Parameter.borrow(ctx, "W", (vocab, hidden), W, dW)
+        X, T, dx = DeviceArray.from_numpy(ctx, x), DeviceArray.from_numpy(ctx, t), DeviceArray(ctx, (rows, hidden))
+        row_loss, lse = DeviceArray(ctx, (rows,)), DeviceArray(ctx, (rows,))
+        ops.vocab_ce(P, None, X, T, rows, row_loss, lse, scale=0.5)
+        ops.vocab_ce_backward(P, None, X, T, rows, lse, dx, scale=0.5)
+        xd, wd, n = x.astype(np.float64), w.astype(np.float64), np.arange(rows)
+        z, at = xd @ wd.T, t - (vocab - last)
+        want = np.log(vocab - last + np.exp(z).sum(1))
+        dz = (12 * U + hidden * U) * (np.abs(xd) @ np.abs(wd).T) + 2 * U * np.abs(z)
+        off = dz.max(1) + 8 * U * (1 + np.abs(want))
+        assert (np.abs(lse.numpy() - want) <= off).all()
+        assert (np.abs(row_loss.numpy() - (want - z[n, at])) <= off + dz[n, at] + 8 * U * np.abs(want)).all()
+        p = np.exp(z - want[:, None])
+        G = 0.5 * p
+        G[n, at] -= 0.5
+        dG = 0.5 * p * (dz + off[:, None] + 4 * U * (2 + np.abs(z - want[:, None]))) + 4 * U * np.abs(G) + 2.0 ** -38
+        sums = lambda a, b, k: (12 + k) * U * (np.abs(a) @ np.abs(b))  # noqa: E731
+        assert (np.abs(dx.numpy() - G @ wd) <= dG @ np.abs(wd) + sums(G, wd, 2 * last) + 4 * U * np.abs(G @ wd)).all()
+        got = part(dW, vocab - last).numpy()
+        assert (np.abs(got - G.T @ xd) <= dG.T @ np.abs(xd) + sums(G.T, xd, rows) + 4 * U * np.abs(G.T @ xd)).all()
+        G0 = 0.5 * np.exp(-want)[:, None] * np.ones(last)  # rows of zeros, one side and the other of 2^31 values
+        dG0 = G0 * (off[:, None] + 4 * U * (2 + np.abs(want[:, None]))) + 2.0 ** -38
+        for v in (0, 2 ** 31 // hidden - last // 2, vocab - 2 * last):
+            got = part(dW, v).numpy()
+            assert (np.abs(got - G0.T @ xd) <= dG0.T @ np.abs(xd) + sums(G0.T, xd, rows) + 4 * U * np.abs(G0.T @ xd)).all()
+    finally:
+        W.free()
+        dW.free()
+
+
 @pytest.mark.parametrize("rows", [24, 280])
 def test_gradient_against_differences_of_the_loss(ctx, rows):
     """Central differences of the device's own loss along random directions. With step h the quotient is off by
