@@ -576,6 +576,7 @@ __global__ __launch_bounds__(256) void few_dx_sum_kernel(const float* __restrict
         const float* at = part + (size_t)j * hidden + h;
         const size_t next = (size_t)pitch * hidden;
         int k = 0;
+#pragma unroll 4
         for (; k + 3 < slices; k += 4)
 #pragma unroll
             for (int q = 0; q < 4; ++q) s[q] += at[(k + q) * next];
